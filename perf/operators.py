@@ -250,7 +250,8 @@ def _quantise(x, bits):
     """fp32 [..., D] -> (c [..., D/8, 8] int32, h [..., D/8] bool, beta [...] fp32)."""
     top = 7 - 2.0 ** -19 if bits == 4 else 127 - 2.0 ** -15
     amax = x.abs().amax(-1)
-    up = (((amax / top).view(torch.int32) + 0xffff) & -0x10000).view(torch.float32)
+    # divided by a tensor: by a Python number it is a product with the reciprocal
+    up = (((amax / torch.full_like(amax, top)).view(torch.int32) + 0xffff) & -0x10000).view(torch.float32)
     small = amax < 2.0 ** -64
     fine = (amax >= 2.0 ** -64) & (amax <= 2.0 ** 64)
     beta = torch.where(fine, up, torch.where(small, 0.0, math.nan))
@@ -522,9 +523,9 @@ def _exact_nearest(x, bits):
     x = x.double()
     amax = x.abs().amax(-1, keepdim=True)
     beta = amax / (7 - 2.0 ** -19 if bits == 4 else 127 - 2.0 ** -15)
-    # up to 8 significant bits
-    unit = torch.pow(2.0, torch.floor(torch.log2(beta)) - 7)
-    beta = torch.ceil(beta / unit) * unit
+    # up to 8 significant bits: 45 of the 52 stored ones cleared
+    rest = (1 << 45) - 1
+    beta = ((beta.view(torch.int64) + rest) & ~rest).view(torch.float64)
     x, scale = x.unflatten(-1, (-1, 8)), beta[..., None]
     whole = torch.round(x / scale)
     away = (x - whole * scale).abs()
