@@ -47,6 +47,8 @@ from .vlut import (
     PreparedWords,
 )
 
+from .kvcache import E8KVCache, draft_tree_mask, kv_attention, kv_read, kv_write
+from .rope import qk_norm_rope, rope_table
 from . import legacy  # coset.legacy.quant.functional: encode / decode / quantize with the overload loop
 from .packed import PackedLinear, load_packed, packed_state, save_packed
 
@@ -61,5 +63,6 @@ __all__ = [
     "E8WeightQuant", "E8ThetaWeightQuant", "D4ThetaWeightQuant", "create_d4_hnlq_linear", "create_e8_hnlq_linear", "get_generators", "ste_quantize",
     "vLUTManager", "QuantizationConfig", "build_vlut", "_encoding_to_index", "vlut_mac_operation",
     "vlut_accumulate_operation", "build_one_sided_vluts", "vlut_dot", "vlut_matmul", "vlut_prepare", "PreparedWords",
+    "E8KVCache", "kv_write", "kv_read", "kv_attention", "draft_tree_mask", "qk_norm_rope", "rope_table",
     "legacy", "PackedLinear", "load_packed", "packed_state", "save_packed",
 ]

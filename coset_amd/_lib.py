@@ -74,6 +74,12 @@ SIGNATURES = {
     "coset_probe_read": [_vp, _i64, _int, _int, _vp, _vp],
     "coset_probe_c2_stream": [_vp, _i64, _vp, _vp, _int, _vp],
     "coset_probe_valu": [_int, _int, _int, _vp, _vp],
+    "coset_kv_write": [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _int, _vp, _i64, _vp],
+    "coset_kv_read": [_vp, _vp, _i64, _vp, _vp, _int, _vp],
+    "coset_kv_attention": [_vp, _vp, _i64, _i64, _int, _i64, _int, _int, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _flt,
+                           _vp, _vp, _vp, _i64, _vp],
+    "coset_qk_norm_rope_fwd": [_vp, _vp, _vp, _vp],
+    "coset_qk_norm_rope_bwd": [_vp, _vp, _vp, _vp, _i64, _vp],
     "coset_init": [_int],
     "coset_set_option": [_int, _int],
 }
@@ -87,6 +93,8 @@ SIZE_QUERIES = {
     "coset_gemm_tn_workspace_floats": [_i64, _i64, _i64],
     "coset_gemm_wgrad_workspace_floats": [_i64, _i64, _i64],
     "coset_vlut_noalloc_scratch_floats": [],
+    "coset_kv_attention_workspace_floats": [_vp, _i64, _int, _int, _int, _i64],
+    "coset_qk_norm_rope_workspace_floats": [_i64, _int],
 }
 
 OPT_CODEC_PATH = 1
@@ -100,6 +108,29 @@ OPT_GEMM_TN_TILE = 8
 OPT_VLUT_GEMM = 9
 OPT_GEMM_WGRAD = 10
 CODEC_AUTO, CODEC_GENERIC, CODEC_LUT = 0, 1, 2
+
+
+
+class KvCacheStruct(ctypes.Structure):
+    """coset_kv_cache"""
+    _fields_ = [("k", _vp), ("v", _vp), ("scales", _vp), ("pages", _i64), ("page_size", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("bits", ctypes.c_int32)]
+
+
+class RopeSideStruct(ctypes.Structure):
+    """coset_rope_side"""
+    _fields_ = [("x", _vp), ("grad", _vp), ("out", _vp), ("weight", _vp), ("weight_grad", _vp),
+                ("token_stride", _i64), ("head_stride", _i64), ("grad_token_stride", _i64),
+                ("grad_head_stride", _i64), ("heads", _i64)]
+
+
+class RopeStruct(ctypes.Structure):
+    """coset_rope"""
+    _fields_ = [("table", _vp), ("positions", _vp), ("n", _i64), ("length", _i64), ("pos_stride", _i64),
+                ("dim", ctypes.c_int32), ("rot", ctypes.c_int32), ("axes", ctypes.c_int32),
+                ("bounds", ctypes.c_int32 * 4), ("norm", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("w_dtype", ctypes.c_int32), ("eps", _flt)]
+
 
 _lib = None
 

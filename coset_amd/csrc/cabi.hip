@@ -12,8 +12,11 @@
 #include "../../include/coset_amd.h"
 #include "codec_kernels.hpp"
 #include "gemm.hpp"
+#include "kv_attention.hpp"
+#include "kv_cache.hpp"
 #include "legacy.hpp"
 #include "probes.hpp"
+#include "qk_rope.hpp"
 #include "tables.hpp"
 #include "vlut.hpp"
 
@@ -894,6 +897,252 @@ int coset_e8_lattice_op(int op, int legacy, const float* in, int64_t n_blocks, i
     if (op == COSET_OP_ENCODE_COORDS && q < 1) return fail(COSET_EINVAL, "q must be positive");
     return check_hip(coset::launch_lattice_op(op, legacy, in, n_blocks, q, out, (hipStream_t)stream),
                      "lattice op launch");
+}
+
+// ---------------------------------------------------------------- E8 key/value cache, attention, head norms with rotation
+
+static int check_any_dtype(int dt)
+{
+    if (dt != COSET_F32 && dt != COSET_BF16 && dt != COSET_F16)
+        return fail(COSET_EUNSUPPORTED, "dtype %d not supported (fp32, bf16, fp16)", dt);
+    return COSET_OK;
+}
+
+static int64_t dtype_size(int dt) { return dt == COSET_F32 ? 4 : 2; }
+
+// 16-byte loads of 8 (fp32: two of 4) values at any token and head
+static bool rows_aligned(const void* p, int64_t tok, int64_t head, int dt)
+{
+    const int64_t per = 16 / dtype_size(dt);
+    return aligned(p, 16) && tok % per == 0 && head % per == 0;
+}
+
+static int kv_cache_of(const coset_kv_cache* c, coset::KvCache& out)
+{
+    if (!c) return fail(COSET_EINVAL, "NULL cache");
+    if (c->bits != 4 && c->bits != 8) return fail(COSET_EINVAL, "bits must be 4 or 8 (got %d)", c->bits);
+    if (c->page_size < 16 || c->page_size % 16) return fail(COSET_EINVAL, "page_size must be a multiple of 16 (got %d)", c->page_size);
+    if (c->head_dim < 32 || c->head_dim > 256 || c->head_dim % 32)
+        return fail(COSET_EUNSUPPORTED, "head_dim must be a multiple of 32 up to 256 (got %d)", c->head_dim);
+    if (c->kv_heads < 1 || c->kv_heads > 32767) return fail(COSET_EINVAL, "kv_heads=%d outside [1, 32767]", c->kv_heads);
+    if (c->pages < 0) return fail(COSET_EINVAL, "pages < 0");
+    if (c->pages > 0x7fffffff / c->page_size)
+        return fail(COSET_EUNSUPPORTED, "pages * page_size must stay below 2^31 (got %lld * %d)", (long long)c->pages, c->page_size);
+    if (c->pages > 0 && (!c->k || !c->v || !c->scales)) return fail(COSET_EINVAL, "NULL cache buffer");
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->scales, 16))
+        return fail(COSET_EINVAL, "cache buffers must be 16-byte aligned");
+    out.k = (uint32_t*)c->k;
+    out.v = (uint32_t*)c->v;
+    out.scales = (uint32_t*)c->scales;
+    out.pages = (uint32_t)c->pages;
+    out.page_size = (uint32_t)c->page_size;
+    out.heads = (uint32_t)c->kv_heads;
+    out.dim = c->head_dim;
+    out.bits = c->bits;
+    out.page_div = coset::u32div_of((uint32_t)c->page_size);
+    return COSET_OK;
+}
+
+int coset_kv_write(const coset_kv_cache* cache, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                   const void* v, int64_t v_token_stride, int64_t v_head_stride, int dtype, const int64_t* slots,
+                   int64_t n, void* stream)
+{
+    int rc;
+    coset::KvRowsArgs a{};
+    if ((rc = kv_cache_of(cache, a.c))) return rc;
+    if ((rc = check_any_dtype(dtype))) return rc;
+    if (n < 0 || n > 0x7fffffff) return fail(COSET_EINVAL, "n=%lld outside [0, 2^31)", (long long)n);
+    if (n > 0 && (!k || !v || !slots)) return fail(COSET_EINVAL, "NULL buffer");
+    if (!aligned(k, dtype_size(dtype)) || !aligned(v, dtype_size(dtype)) || !aligned(slots, 8))
+        return fail(COSET_EINVAL, "misaligned buffer");
+    a.slots = slots;
+    a.n = n;
+    a.k = k;
+    a.v = v;
+    a.k_tok = k_token_stride;
+    a.k_head = k_head_stride;
+    a.v_tok = v_token_stride;
+    a.v_head = v_head_stride;
+    a.vec = rows_aligned(k, k_token_stride, k_head_stride, dtype) && rows_aligned(v, v_token_stride, v_head_stride, dtype);
+    a.dtype = dtype;
+    return check_hip(coset::launch_kv_write(a, (hipStream_t)stream), "kv write launch");
+}
+
+int coset_kv_read(const coset_kv_cache* cache, const int64_t* slots, int64_t n, void* k, void* v, int dtype,
+                  void* stream)
+{
+    int rc;
+    coset::KvRowsArgs a{};
+    if ((rc = kv_cache_of(cache, a.c))) return rc;
+    if ((rc = check_any_dtype(dtype))) return rc;
+    if (n < 0 || n > 0x7fffffff) return fail(COSET_EINVAL, "n=%lld outside [0, 2^31)", (long long)n);
+    if (n > 0 && (!k || !v || !slots)) return fail(COSET_EINVAL, "NULL buffer");
+    if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 8)) return fail(COSET_EINVAL, "k and v must be 16-byte aligned");
+    a.slots = slots;
+    a.n = n;
+    a.k_out = k;
+    a.v_out = v;
+    a.dtype = dtype;
+    return check_hip(coset::launch_kv_read(a, (hipStream_t)stream), "kv read launch");
+}
+
+static int kv_attention_shape(const coset::KvCache& c, int64_t n, int heads, int seqs, int dtype, int64_t max_pages,
+                              coset::KvAttentionPlan& p)
+{
+    int rc;
+    if ((rc = check_any_dtype(dtype))) return rc;
+    if (n < 0 || seqs < 1 || seqs > (1 << 20) || max_pages < 0) return fail(COSET_EINVAL, "bad shape n=%lld seqs=%d max_pages=%lld", (long long)n, seqs, (long long)max_pages);
+    if (heads < 1 || heads % (int)c.heads)
+        return fail(COSET_EINVAL, "heads=%d is not a multiple of kv_heads=%u", heads, c.heads);
+    if (max_pages > 0x7fffff00 / (int64_t)c.page_size || n > 0x7fffffff / heads)
+        return fail(COSET_EUNSUPPORTED, "max_pages * page_size and n * heads must stay below 2^31");
+    p = coset::kv_attention_plan(n, seqs, heads, (int)c.heads, c.dim, c.bits, dtype, max_pages * c.page_size);
+    if (p.units > (1 << 30)) return fail(COSET_EUNSUPPORTED, "more than 2^30 steps of 128 tokens in one call");
+    return COSET_OK;
+}
+
+int64_t coset_kv_attention_workspace_floats(const coset_kv_cache* cache, int64_t n, int seqs, int heads, int dtype,
+                                            int64_t max_pages)
+{
+    coset::KvCache c;
+    coset::KvAttentionPlan p;
+    if (kv_cache_of(cache, c) || kv_attention_shape(c, n, heads, seqs, dtype, max_pages, p)) return 0;
+    return p.workspace_floats;
+}
+
+int coset_kv_attention(const coset_kv_cache* cache, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                       int dtype, int64_t n, int heads, int seqs, const int32_t* starts, const int32_t* lengths,
+                       const int32_t* block_table, int64_t table_stride, int64_t max_pages, const int64_t* tree_mask,
+                       int64_t mask_words, float scale, void* out, float* lse, float* workspace,
+                       int64_t workspace_floats, void* stream)
+{
+    int rc;
+    coset::KvAttentionArgs a{};
+    coset::KvAttentionPlan p;
+    if ((rc = kv_cache_of(cache, a.c))) return rc;
+    if ((rc = kv_attention_shape(a.c, n, heads, seqs, dtype, max_pages, p))) return rc;
+    if (!starts && n % seqs) return fail(COSET_EINVAL, "n=%lld is not a multiple of seqs=%d", (long long)n, seqs);
+    if (mask_words < 0 || mask_words > (1 << 20)) return fail(COSET_EINVAL, "mask_words=%lld outside [0, 2^20]", (long long)mask_words);
+    if (n == 0) return COSET_OK;
+    if (a.c.pages == 0 || max_pages == 0) return fail(COSET_EINVAL, "a cache and a block table of at least one page are needed");
+    if (!q || !lengths || !block_table || !out || (mask_words > 0 && !tree_mask)) return fail(COSET_EINVAL, "NULL buffer");
+    if (!aligned(q, dtype_size(dtype)) || !aligned(out, 16) || !aligned(tree_mask, 8))
+        return fail(COSET_EINVAL, "misaligned buffer (out needs 16 bytes)");
+    if (!workspace || !aligned(workspace, 16) || workspace_floats < p.workspace_floats)
+        return fail(COSET_EINVAL, "workspace holds %lld floats, needs %lld (16-byte aligned)", (long long)(workspace ? workspace_floats : 0),
+                    (long long)p.workspace_floats);
+    a.q = q;
+    a.q_tok = q_token_stride;
+    a.q_head = q_head_stride;
+    a.vec = rows_aligned(q, q_token_stride, q_head_stride, dtype);
+    a.dtype = dtype;
+    a.heads = heads;
+    a.group = heads / (int)a.c.heads;
+    a.group_div = coset::u32div_of((uint32_t)a.group);
+    a.n = n;
+    a.seqs = seqs;
+    a.starts = starts;
+    a.lengths = lengths;
+    a.table = block_table;
+    a.table_stride = table_stride;
+    a.max_pages = (int)max_pages;
+    a.mask = tree_mask;
+    a.mask_words = (int)mask_words;
+    a.scale = scale * 1.44269504088896340736f;
+    a.out = out;
+    a.lse = lse;
+    a.workspace = workspace;
+    return check_hip(coset::launch_kv_attention(a, p, (hipStream_t)stream), "kv attention launch");
+}
+
+static int rope_of(const coset_rope* r, const coset_rope_side* q, const coset_rope_side* k, bool backward,
+                   coset::RopeArgs& a)
+{
+    int rc;
+    if (!r || !q || !k) return fail(COSET_EINVAL, "NULL argument");
+    if ((rc = check_any_dtype(r->dtype)) || (rc = check_any_dtype(r->w_dtype))) return rc;
+    if (r->n < 0 || r->n > 0x7fffffff) return fail(COSET_EINVAL, "n=%lld outside [0, 2^31)", (long long)r->n);
+    if (r->dim < 8 || r->dim > coset::kRopeMaxDim || r->dim % 8)
+        return fail(COSET_EUNSUPPORTED, "dim must be a multiple of 8 up to %d (got %d)", coset::kRopeMaxDim, r->dim);
+    if (r->rot < 0 || r->rot > r->dim || r->rot % 8)
+        return fail(COSET_EUNSUPPORTED, "rot must be a multiple of 8 up to dim=%d (got %d)", r->dim, r->rot);
+    if (r->axes < 1 || r->axes > coset::kRopeMaxAxes) return fail(COSET_EINVAL, "axes=%d outside [1, %d]", r->axes, coset::kRopeMaxAxes);
+    if (r->n > 0 && r->rot > 0 && (!r->table || !r->positions || r->length < 1))
+        return fail(COSET_EINVAL, "a table of at least one position and positions are needed");
+    if (!aligned(r->table, 16) || !aligned(r->positions, 8)) return fail(COSET_EINVAL, "table must be 16-byte aligned, positions 8-byte");
+    if (!(r->eps >= 0.f)) return fail(COSET_EINVAL, "eps must be >= 0");
+    const coset_rope_side* in[2] = {q, k};
+    coset::RopeSide* out[2] = {&a.q, &a.k};
+    for (int i = 0; i < 2; ++i) {
+        const coset_rope_side& s = *in[i];
+        if (s.heads < 0 || s.heads > 32767) return fail(COSET_EINVAL, "heads=%lld outside [0, 32767]", (long long)s.heads);
+        const bool some = r->n > 0 && s.heads > 0;
+        const bool reads_x = !backward || r->norm;
+        if (some && ((reads_x && !s.x) || !s.out || (backward && !s.grad))) return fail(COSET_EINVAL, "NULL buffer");
+        if (!aligned(s.out, 16) || !aligned(s.x, dtype_size(r->dtype)) || !aligned(s.grad, dtype_size(r->dtype)))
+            return fail(COSET_EINVAL, "misaligned buffer (outputs need 16 bytes)");
+        coset::RopeSide& o = *out[i];
+        o.x = s.x;
+        o.g = s.grad;
+        o.out = s.out;
+        o.w = r->norm ? s.weight : nullptr;
+        o.x_tok = s.token_stride;
+        o.x_head = s.head_stride;
+        o.g_tok = s.grad_token_stride;
+        o.g_head = s.grad_head_stride;
+        o.heads = (int)s.heads;
+        o.vec = (!reads_x || rows_aligned(s.x, s.token_stride, s.head_stride, r->dtype)) &&
+                (!backward || rows_aligned(s.grad, s.grad_token_stride, s.grad_head_stride, r->dtype));
+    }
+    if (q->heads + k->heads < 1) return fail(COSET_EINVAL, "no heads");
+    a.table = r->table;
+    a.pos = r->positions;
+    a.n = r->n;
+    a.length = r->length;
+    a.pos_axis = r->pos_stride;
+    a.dim = r->dim;
+    a.rot = r->rot;
+    a.axes = r->axes;
+    for (int i = 0; i < coset::kRopeMaxAxes; ++i) a.bound[i] = r->bounds[i];
+    a.norm = r->norm ? 1 : 0;
+    a.interleaved = r->interleaved ? 1 : 0;
+    a.dtype = r->dtype;
+    a.w_dtype = r->w_dtype;
+    a.eps = r->eps;
+    return COSET_OK;
+}
+
+int coset_qk_norm_rope_fwd(const coset_rope* r, const coset_rope_side* q, const coset_rope_side* k, void* stream)
+{
+    coset::RopeArgs a{};
+    int rc = rope_of(r, q, k, false, a);
+    if (rc) return rc;
+    return check_hip(coset::launch_rope_fwd(a, (hipStream_t)stream), "norm and rotation launch");
+}
+
+int64_t coset_qk_norm_rope_workspace_floats(int64_t n, int dim)
+{
+    if (n < 0 || dim < 8 || dim > coset::kRopeMaxDim) return 0;
+    return (int64_t)coset::rope_bwd_groups(n, dim) * 2 * dim;
+}
+
+int coset_qk_norm_rope_bwd(const coset_rope* r, const coset_rope_side* q, const coset_rope_side* k, float* workspace,
+                           int64_t workspace_floats, void* stream)
+{
+    coset::RopeArgs a{};
+    int rc = rope_of(r, q, k, true, a);
+    if (rc) return rc;
+    if (q->weight_grad || k->weight_grad) {
+        if (!a.norm) return fail(COSET_EINVAL, "weight gradients without the norm");
+        const int64_t need = coset_qk_norm_rope_workspace_floats(r->n, r->dim);
+        if (need > 0 && !workspace) return fail(COSET_EINVAL, "NULL workspace");
+        if (workspace_floats < need)
+            return fail(COSET_EINVAL, "workspace holds %lld floats, needs %lld", (long long)workspace_floats, (long long)need);
+        a.gw_q = q->weight_grad;
+        a.gw_k = k->weight_grad;
+        a.partial = workspace;
+    }
+    return check_hip(coset::launch_rope_bwd(a, (hipStream_t)stream), "norm and rotation backward launch");
 }
 
 // ---------------------------------------------------------------- measurement probes

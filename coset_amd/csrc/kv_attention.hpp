@@ -1,0 +1,49 @@
+// kv_attention.hpp -- attention of new tokens over the E8 key/value cache
+// (kv_attention.hip; cache format: kv_cache.hpp).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "kv_cache.hpp"
+
+namespace coset {
+
+struct KvAttentionArgs {
+    KvCache c;
+    const void* q;             // [n, heads, dim], strides in elements
+    int64_t q_tok, q_head;
+    int vec;                   // q may be read 16 bytes at a time
+    int dtype;                 // of q and out
+    int heads;                 // query heads; group = heads / c.heads of them share a key head
+    int group;
+    U32Div group_div;
+    int64_t n;                 // query tokens
+    int seqs;
+    const int32_t* starts;     // [seqs + 1] first query token of each sequence, or NULL: n / seqs each
+    const int32_t* lengths;    // [seqs] cached tokens, the sequence's new ones last
+    const int32_t* table;      // [seqs, max_pages]
+    int64_t table_stride;
+    int max_pages;
+    const int64_t* mask;       // [n, mask_words] bit j: the sequence's new token j is seen; NULL: j <= own
+    int mask_words;
+    float scale;               // times log2(e)
+    void* out;                 // [n, heads, dim] contiguous
+    float* lse;                // [n, heads] or NULL
+    float* workspace;
+};
+
+// How a call is cut: `rows` query rows (token x head of a group) per
+// workgroup, at most `blocks` workgroups.
+struct KvAttentionPlan {
+    int tiles;      // 16-row tiles a workgroup holds: 1, 2 or 4
+    int blocks;
+    int pad_dim;    // 64, 128 or 256
+    int64_t units;  // steps of 128 tokens at most
+    int64_t workspace_floats;
+};
+KvAttentionPlan kv_attention_plan(int64_t n, int seqs, int heads, int kv_heads, int dim, int bits, int dtype,
+                                  int64_t max_tokens);
+hipError_t launch_kv_attention(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_t s);
+
+}  // namespace coset

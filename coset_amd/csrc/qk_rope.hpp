@@ -1,0 +1,42 @@
+// qk_rope.hpp -- RMS norm of each head's query and key and the position
+// rotation in one pass, and its backward (qk_rope.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace coset {
+
+constexpr int kRopeMaxAxes = 4;
+constexpr int kRopeMaxDim = 512;
+
+struct RopeSide {           // the queries or the keys
+    const void* x;          // [n, heads, dim], strides in elements
+    const void* g;          // backward: gradient of the output
+    void* out;              // [n, heads, dim] contiguous: the output, or the gradient of x
+    const void* w;          // [dim] norm weights or NULL (no weight: ones)
+    int64_t x_tok, x_head, g_tok, g_head;
+    int heads;
+    int vec;                // x (and g) may be read 16 bytes at a time
+};
+
+struct RopeArgs {
+    RopeSide q, k;
+    const float* table;     // [length, rot]: cosines of the rot/2 pairs, then their sines
+    const int64_t* pos;     // [axes, n], clamped to [0, length)
+    int64_t n, length, pos_axis;   // pos_axis: elements from one axis's positions to the next
+    int dim, rot, axes;
+    int bound[kRopeMaxAxes];   // pair i turns by axis a, the first with i < bound[a]
+    int norm, interleaved;
+    int dtype, w_dtype;
+    float eps;
+    float* partial;         // backward: [groups, 2, dim] sums for the weights' gradients
+    void* gw_q;             // backward: [dim] in w_dtype, nullable
+    void* gw_k;
+};
+
+hipError_t launch_rope_fwd(const RopeArgs& a, hipStream_t s);
+hipError_t launch_rope_bwd(const RopeArgs& a, hipStream_t s);
+int rope_bwd_groups(int64_t n, int dim);
+
+}  // namespace coset

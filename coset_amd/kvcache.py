@@ -1,0 +1,239 @@
+"""Keys and values of attention kept as points of the E8 lattice, 4 or 8 bits a value, and attention over them.
+
+A head's vector x of D values is held as x_hat = beta lambda: a bf16 scale
+beta = max|x| / C rounded up (C a little below 7 or 127) and D / 8 points
+lambda of E8, each the nearest to its 8 values over beta.  beta is never small
+enough for a point to leave the range that the bits hold, so nothing is ever
+clipped; a block of 8 takes 32 or 64 bits and is read back without a table
+(E8 = D8 + {0, 1/2}: eight integers with an even sum, and one half for all of
+them whose bit stands where the sum's parity makes one redundant).  The mean
+squared error is that of rounding each value at the same scale, less about
+12 %.
+
+The cache is paged: a row is page * page_size + offset, a sequence the rows
+of its pages in the order of its block table.  The kernels are behind
+coset_kv_* in include/coset_amd.h, which states the words' layout; the
+reference has no such cache.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+class E8KVCache:
+    """A paged cache's tensors:
+
+      k       int32 [pages, kv_heads, page_size, head_dim / 8 * w]       w = bits / 4
+      v       int32 [pages, kv_heads, page_size / 4, head_dim / 8, 4, w]
+      scales  bfloat16 [pages, kv_heads, page_size, 2]                   the key's and the value's
+
+    ``E8KVCache.empty`` allocates them; the constructor takes tensors that
+    exist (those of a saved cache, say), contiguous and on one GPU.
+    head_dim: a multiple of 32 up to 256; page_size: a multiple of 16.
+    """
+
+    __slots__ = ("k", "v", "scales", "bits", "pages", "page_size", "kv_heads", "head_dim", "_struct", "_ref")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor, bits: int = 4):
+        if bits not in (4, 8):
+            raise ValueError(f"bits must be 4 or 8, got {bits}")
+        if k.dim() != 4:
+            raise ValueError(f"k must be [pages, kv_heads, page_size, words], got {tuple(k.shape)}")
+        pages, heads, page, words = k.shape
+        w = bits // 4
+        if words % w or v.shape != (pages, heads, page // 4, words // w, 4, w) or scales.shape != (pages, heads, page, 2):
+            raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)} and scales {tuple(scales.shape)} are not the "
+                             f"tensors of one {bits}-bit cache")
+        if k.dtype != torch.int32 or v.dtype != torch.int32 or scales.dtype != torch.bfloat16:
+            raise ValueError("k and v must be int32, scales bfloat16")
+        if not (k.is_contiguous() and v.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("cache tensors must be contiguous")
+        if k.device != v.device or k.device != scales.device:
+            raise ValueError("cache tensors must be on one device")
+        self.k, self.v, self.scales, self.bits = k, v, scales, bits
+        self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, page, words // w * 8
+        self._struct = _lib.KvCacheStruct(k.data_ptr(), v.data_ptr(), scales.data_ptr(), pages, page, heads,
+                                          self.head_dim, bits)
+        self._ref = ctypes.addressof(self._struct)
+
+    @classmethod
+    def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int = 4,
+              device: Optional[torch.device] = None) -> "E8KVCache":
+        """A cache whose rows all read back as zeros."""
+        if page_size < 16 or page_size % 16:
+            raise ValueError(f"page_size must be a multiple of 16, got {page_size}")
+        if head_dim < 32 or head_dim > 256 or head_dim % 32:
+            raise ValueError(f"head_dim must be a multiple of 32 up to 256, got {head_dim}")
+        if bits not in (4, 8):
+            raise ValueError(f"bits must be 4 or 8, got {bits}")
+        dev = _lib.require_gpu() if device is None else torch.device(device)
+        w, nb = bits // 4, head_dim // 8
+        return cls(torch.zeros((pages, kv_heads, page_size, nb * w), dtype=torch.int32, device=dev),
+                   torch.zeros((pages, kv_heads, page_size // 4, nb, 4, w), dtype=torch.int32, device=dev),
+                   torch.zeros((pages, kv_heads, page_size, 2), dtype=torch.bfloat16, device=dev), bits)
+
+    def nbytes(self) -> int:
+        return 4 * (self.k.numel() + self.v.numel()) + 2 * self.scales.numel()
+
+
+def _dtype(dt: torch.dtype) -> int:
+    code = _DTYPES.get(dt)
+    if code is None:
+        raise ValueError(f"unsupported dtype {dt} (float32, bfloat16 or float16)")
+    return code
+
+
+def _on_device(cache: E8KVCache, **tensors) -> torch.device:
+    dev = cache.k.device
+    if dev.type != "cuda":
+        raise _lib.CosetError("the cache is not on a GPU")
+    for name, t in tensors.items():
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+    return dev
+
+
+def _slots(slots: torch.Tensor, n: Optional[int]) -> torch.Tensor:
+    if slots.dim() != 1 or (n is not None and slots.shape[0] != n):
+        raise ValueError(f"slots must be a vector of {'rows' if n is None else n}, got {tuple(slots.shape)}")
+    if slots.dtype != torch.int64:
+        if slots.dtype != torch.int32:
+            raise ValueError("slots must be int64 (or int32)")
+        slots = slots.long()
+    return slots.contiguous()
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
+def kv_write(cache: E8KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantize k and v [n, kv_heads, head_dim] (fp32, bf16 or fp16; any
+    strides with contiguous heads) into the cache's rows ``slots`` [n].
+
+    A row is page * page_size + offset; rows outside the cache (-1, say, for
+    padding) are skipped.  Rows must not repeat within one call.  A vector
+    with an infinity or a NaN reads back as NaN, one whose largest magnitude
+    is below 2^-64 as zeros.  Not differentiable."""
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != cache.kv_heads or k.shape[2] != cache.head_dim:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [n, {cache.kv_heads}, {cache.head_dim}]")
+    if k.dtype != v.dtype:
+        raise ValueError(f"k is {k.dtype}, v {v.dtype}")
+    dt = _dtype(k.dtype)
+    dev = _on_device(cache, k=k, v=v, slots=slots)
+    n = k.shape[0]
+    slots = _slots(slots, n)
+    k, v = _rows(k), _rows(v)
+    with torch.cuda.device(dev):
+        _lib.call("coset_kv_write", cache._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                  v.stride(1), dt, slots.data_ptr(), n, _lib.stream_of(k))
+
+
+def kv_read(cache: E8KVCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16
+            ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values in rows ``slots`` [n], each [n, kv_heads, head_dim]
+    in ``dtype`` (beta lambda in fp32, rounded once).  Rows outside the cache
+    are zeros."""
+    dt = _dtype(dtype)
+    dev = _on_device(cache, slots=slots)
+    slots = _slots(slots, None)
+    n = slots.shape[0]
+    with torch.cuda.device(dev):
+        k = torch.empty((n, cache.kv_heads, cache.head_dim), dtype=dtype, device=dev)
+        v = torch.empty_like(k)
+        _lib.call("coset_kv_read", cache._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), dt,
+                  _lib.stream_of(k))
+    return k, v
+
+
+def draft_tree_mask(parents: Union[torch.Tensor, Sequence[int]]) -> torch.Tensor:
+    """parents [T] or [seqs, T]: the drafted token that each one follows (an
+    earlier one of its sequence), or a negative number for one that follows
+    the cached context.  Returns kv_attention's ``tree_mask`` rows
+    [T, words] or [seqs, T, words] (int64): a token sees itself and the tokens
+    on its path."""
+    p = torch.as_tensor(parents)
+    flat = (p if p.dim() == 2 else p[None]).cpu().long()
+    seqs, T = flat.shape
+    if bool((flat >= torch.arange(T)).any()):
+        raise ValueError("a drafted token must follow an earlier one")
+    seen = torch.eye(T, dtype=torch.bool).expand(seqs, T, T).clone()
+    at = torch.arange(seqs)
+    for t in range(T):
+        up = flat[:, t]
+        seen[:, t] |= seen[at, up.clamp(min=0)] & (up >= 0)[:, None]
+    words = max(-(-T // 64), 1)
+    bits = torch.zeros((seqs, T, words * 64), dtype=torch.int64)
+    bits[:, :, :T] = seen
+    out = (bits.view(seqs, T, words, 64) << torch.arange(64)).sum(-1)
+    return (out if p.dim() == 2 else out[0]).to(p.device)
+
+
+def kv_attention(q: torch.Tensor, cache: E8KVCache, block_table: torch.Tensor, lengths: torch.Tensor, *,
+                 cu_queries: Optional[torch.Tensor] = None, tree_mask: Optional[torch.Tensor] = None,
+                 scale: Optional[float] = None, return_lse: bool = False, workspace: Optional[torch.Tensor] = None
+                 ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Attention of new tokens over the cache, which already holds their own
+    keys and values.
+
+    q: [n, heads, head_dim] fp32, bf16 or fp16, the sequences' new tokens one
+    after another; heads is a multiple of the cache's (query head h reads key
+    head h // (heads / kv_heads)).  block_table: int32 [seqs, max_pages], a
+    sequence's pages in order.  lengths: int32 [seqs], a sequence's cached
+    tokens, its new ones the last.  cu_queries: int32 [seqs + 1], each
+    sequence's first new token; None: n / seqs each (one for plain decoding).
+
+    A new token sees every cached token before the new ones and, of the new
+    ones, those up to itself, or with ``tree_mask`` int64 [n, words] those
+    whose bits its row sets (draft_tree_mask builds it).  scale: of q . k,
+    head_dim ** -0.5 by default.  Returns out (q's shape and dtype), and with
+    return_lse the log of the softmax's denominator, fp32 [n, heads]; a token
+    that sees nothing gives zeros and -inf.  Not differentiable.
+
+    workspace: fp32 scratch kept between calls on one stream (allocated where
+    it is None or too small)."""
+    if q.dim() != 3 or q.shape[2] != cache.head_dim:
+        raise ValueError(f"q must be [n, heads, {cache.head_dim}], got {tuple(q.shape)}")
+    n, heads, dim = q.shape
+    dt = _dtype(q.dtype)
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        raise ValueError("block_table must be int32 [seqs, max_pages] with contiguous rows")
+    seqs, max_pages = block_table.shape
+    if lengths.shape != (seqs,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+        raise ValueError(f"lengths must be a contiguous int32 vector of {seqs}")
+    dev = _on_device(cache, q=q, block_table=block_table, lengths=lengths)
+    if cu_queries is not None:
+        if cu_queries.shape != (seqs + 1,) or cu_queries.dtype != torch.int32 or not cu_queries.is_contiguous():
+            raise ValueError(f"cu_queries must be a contiguous int32 vector of {seqs + 1}")
+        if cu_queries.device != dev:
+            raise ValueError(f"cu_queries is on {cu_queries.device}, the cache on {dev}")
+    words = 0
+    if tree_mask is not None:
+        if tree_mask.dim() != 2 or tree_mask.shape[0] != n or tree_mask.shape[1] < 1 or \
+                tree_mask.dtype != torch.int64 or not tree_mask.is_contiguous():
+            raise ValueError(f"tree_mask must be contiguous int64 [{n}, words]")
+        if tree_mask.device != dev:
+            raise ValueError(f"tree_mask is on {tree_mask.device}, the cache on {dev}")
+        words = tree_mask.shape[1]
+    q = _rows(q)
+    with torch.cuda.device(dev):
+        out = torch.empty((n, heads, dim), dtype=q.dtype, device=dev)
+        lse = torch.empty((n, heads), dtype=torch.float32, device=dev) if return_lse else None
+        need = _lib.load().coset_kv_attention_workspace_floats(cache._ref, n, seqs, heads, dt, max_pages)
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(need, dtype=torch.float32, device=dev)
+        elif workspace.device != dev or workspace.dtype != torch.float32 or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous fp32 on the cache's device")
+        _lib.call("coset_kv_attention", cache._ref, q.data_ptr(), q.stride(0), q.stride(1), dt, n, heads, seqs,
+                  None if cu_queries is None else cu_queries.data_ptr(), lengths.data_ptr(), block_table.data_ptr(),
+                  block_table.stride(0), max_pages, None if tree_mask is None else tree_mask.data_ptr(), words,
+                  dim ** -0.5 if scale is None else float(scale), out.data_ptr(), _lib.ptr(lse),
+                  workspace.data_ptr(), workspace.numel(), _lib.stream_of(q))
+    return (out, lse) if return_lse else out

@@ -1,0 +1,169 @@
+"""RMS norm of each head's query and key and the position rotation, in one pass, with its gradient.
+
+The kernels are coset_qk_norm_rope_* in include/coset_amd.h; the reference
+has no attention.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+from .kvcache import _dtype, _rows
+
+
+def rope_table(length: int, rot: int, base: float = 10000.0, device: Optional[torch.device] = None) -> torch.Tensor:
+    """[length, rot] fp32: the cosines of position * base^(-2i / rot) for the
+    rot / 2 pairs i, then their sines (computed in 64 bits)."""
+    if rot < 8 or rot % 8:
+        raise ValueError(f"rot must be a positive multiple of 8, got {rot}")
+    dev = _lib.require_gpu() if device is None else torch.device(device)
+    freq = torch.tensor([float(base) ** (-i / rot) for i in range(0, rot, 2)], dtype=torch.float64, device=dev)
+    angle = torch.arange(length, dtype=torch.float64, device=dev)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float()
+
+
+def _side(x, out, weight, grad=None, weight_grad=None):
+    return _lib.RopeSideStruct(
+        x.data_ptr(), None if grad is None else grad.data_ptr(), out.data_ptr(),
+        None if weight is None else weight.data_ptr(), None if weight_grad is None else weight_grad.data_ptr(),
+        x.stride(0), x.stride(1), 0 if grad is None else grad.stride(0), 0 if grad is None else grad.stride(1),
+        x.shape[1])
+
+
+def _plan(q, table, positions, wq, wk, eps, bounds, interleaved, norm):
+    w = wq if wq is not None else wk
+    return _lib.RopeStruct(
+        table.data_ptr(), positions.data_ptr(), q.shape[0], table.shape[0], positions.stride(0), q.shape[2],
+        table.shape[1], positions.shape[0], bounds, norm, interleaved, _dtype(q.dtype),
+        _lib.F32 if w is None else _dtype(w.dtype), eps)
+
+
+def _forward(q, k, table, positions, wq, wk, eps, bounds, interleaved, norm):
+    with torch.cuda.device(q.device):
+        oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        r = _plan(q, table, positions, wq, wk, eps, bounds, interleaved, norm)
+        sq, sk = _side(q, oq, wq), _side(k, ok, wk)
+        _lib.call("coset_qk_norm_rope_fwd", ctypes.addressof(r), ctypes.addressof(sq), ctypes.addressof(sk),
+                  _lib.stream_of(q))
+    return oq, ok
+
+
+class _NormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, table, positions, eps, bounds, interleaved, norm):
+        ctx.save_for_backward(q, k, wq, wk, table, positions)
+        ctx.rest = (eps, bounds, interleaved, norm)
+        return _forward(q, k, table, positions, wq, wk, eps, bounds, interleaved, norm)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, wq, wk, table, positions = ctx.saved_tensors
+        eps, bounds, interleaved, norm = ctx.rest
+        gq, gk = _rows(gq), _rows(gk)
+        with torch.cuda.device(q.device):
+            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
+            dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
+            need = 0
+            ws = None
+            if dwq is not None or dwk is not None:
+                need = _lib.load().coset_qk_norm_rope_workspace_floats(q.shape[0], q.shape[2])
+                ws = torch.empty(need, dtype=torch.float32, device=q.device)
+            r = _plan(q, table, positions, wq, wk, eps, bounds, interleaved, norm)
+            sq, sk = _side(q, dq, wq, gq, dwq), _side(k, dk, wk, gk, dwk)
+            _lib.call("coset_qk_norm_rope_bwd", ctypes.addressof(r), ctypes.addressof(sq), ctypes.addressof(sk),
+                      _lib.ptr(ws), need, _lib.stream_of(q))
+        return dq, dk, dwq, dwk, None, None, None, None, None, None
+
+
+_BOUNDS = {}
+
+
+def _bounds(sections: Tuple[int, ...]):
+    """ctypes int32[4]: the first pair behind each axis's section."""
+    b = _BOUNDS.get(sections)
+    if b is None:
+        at, ends = 0, []
+        for s in sections:
+            at += s
+            ends.append(at)
+        b = _BOUNDS[sections] = (ctypes.c_int32 * 4)(*ends)
+    return b
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, positions: torch.Tensor,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, *,
+                 eps: float = 1e-6, sections: Optional[Sequence[int]] = None, interleaved: bool = False,
+                 norm: Optional[bool] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Queries q [n, heads, dim] and keys k [n, kv_heads, dim] (fp32, bf16 or
+    fp16; any strides with contiguous heads), each head's vector normalized
+    and its first table.shape[1] values rotated by the token's position:
+
+      z = x (mean(x^2) + eps)^(-1/2) weight
+      (z_a cos - z_b sin, z_b cos + z_a sin) for each pair (a, b) of z
+
+    table: rope_table's [length, rot] fp32.  positions: int64 [n], or
+    [axes, n] for positions with several axes (time, height, width): pair i
+    turns by the axis in whose section it lies, ``sections`` holding the
+    axes' numbers of pairs (their sum is rot / 2).  Positions are clamped to
+    the table.  Pairs are (i, i + rot/2), or (2i, 2i + 1) with
+    ``interleaved``.  weights: [dim] in one dtype; None is a weight of ones,
+    and both None leaves the norm out unless ``norm`` is True.  dim and rot
+    are multiples of 8, dim at most 512.
+
+    Differentiable in q, k and the weights (once)."""
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must be [n, heads, dim] with one n and dim")
+    if q.dtype != k.dtype:
+        raise ValueError(f"q is {q.dtype}, k {k.dtype}")
+    _dtype(q.dtype)
+    n, _, dim = q.shape
+    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+        raise ValueError("table must be contiguous fp32 [length, rot]")
+    rot = table.shape[1]
+    if rot > dim or rot % 8 or dim % 8:
+        raise ValueError(f"dim {dim} and rot {rot} must be multiples of 8, rot at most dim")
+    if positions.dim() == 1:
+        positions = positions[None]
+    if positions.dim() != 2 or positions.shape[1] != n or positions.dtype != torch.int64:
+        raise ValueError(f"positions must be int64 [{n}] or [axes, {n}], got {positions.dtype} {tuple(positions.shape)}")
+    axes = positions.shape[0]
+    if sections is None:
+        if axes != 1:
+            raise ValueError("positions of several axes need sections")
+        sections = (rot // 2,)
+    else:
+        sections = tuple(sections)
+        if len(sections) != axes or sum(sections) != rot // 2 or min(sections) < 0:
+            raise ValueError(f"sections {sections} must hold {axes} numbers of pairs with the sum {rot // 2}")
+    if axes > 4:
+        raise ValueError("at most 4 position axes")
+    dev = q.device
+    if dev.type != "cuda":
+        raise _lib.CosetError("q is not on a GPU")
+    if not (k.device == dev and table.device == dev and positions.device == dev):
+        raise ValueError(f"k, table and positions must be on q's device {dev}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.shape != (dim,) or not w.is_contiguous() or w.device != dev):
+            raise ValueError(f"{name} must be a contiguous vector of {dim} on {dev}")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError("the weights must have one dtype")
+    weighted = q_weight is not None or k_weight is not None
+    if norm is None:
+        norm = weighted
+    elif not norm and weighted:
+        raise ValueError("weights without the norm")
+    if positions.stride(1) != 1:
+        positions = positions.contiguous()
+    q, k = _rows(q), _rows(k)
+    args = (float(eps), _bounds(sections), int(bool(interleaved)), int(bool(norm)))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
+                                    (weighted and any(w is not None and w.requires_grad for w in (q_weight, k_weight)))):
+        return _NormRope.apply(q, k, q_weight, k_weight, table, positions, *args)
+    return _forward(q, k, table, positions, q_weight, k_weight, *args)

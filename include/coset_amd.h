@@ -440,6 +440,102 @@ int coset_vlut_linear(const void* words, int word_format, const float* scale, in
                       const float* bias, const float* lsq_alpha, int lsq_qmax, float* workspace,
                       int64_t workspace_floats, float* out, void* stream);
 
+/* Keys and values kept as points of E8 (no reference counterpart).  A head's
+ * vector x of head_dim values is beta lambda: one bf16 scale beta = max|x| / C
+ * rounded up (C = 7 - 2^-19 at 4 bits, 127 - 2^-15 at 8) and head_dim / 8
+ * points lambda of E8, each the nearest to its 8 values over beta.  Every
+ * coordinate is c + h / 2 with c in [-2^(bits-1), 2^(bits-1) - 1] and one h in
+ * {0, 1} for the block; field j of a block (bits bits, from the lowest) is
+ * c_j + 2^(bits-1), and since sum c is even the lowest bit of c_7 follows from
+ * the others and its place holds h.  With w = bits / 4 words of 32 bits a block:
+ *   k       [pages, kv_heads, page_size, head_dim/8, w]          16-byte aligned
+ *   v       [pages, kv_heads, page_size/4, head_dim/8, 4, w]     16-byte aligned
+ *   scales  [pages, kv_heads, page_size, 2] bf16, the key's and the value's
+ * Vectors below 2^-64 in magnitude are kept as zeros; one above 2^64, or with
+ * an infinity or a NaN, reads back as NaN.  bits 4 or 8, page_size a multiple
+ * of 16, head_dim a multiple of 32 up to 256, pages * page_size < 2^31. */
+typedef struct coset_kv_cache {
+    void* k;
+    void* v;
+    void* scales;
+    int64_t pages;
+    int32_t page_size, kv_heads, head_dim, bits;
+} coset_kv_cache;
+
+/* Rows slots[i] = page * page_size + offset (int64, on the device) of the
+ * cache: k and v [n, kv_heads, head_dim] (fp32, bf16 or fp16; strides in
+ * elements, the last dimension contiguous) are quantized into them, or read
+ * from them (contiguous outputs).  A slot outside the cache is skipped, or
+ * read as zeros; a slot named twice in one write keeps either vector, its
+ * words and scale possibly of different ones. */
+int coset_kv_write(const coset_kv_cache* cache, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                   const void* v, int64_t v_token_stride, int64_t v_head_stride, int dtype, const int64_t* slots,
+                   int64_t n, void* stream);
+int coset_kv_read(const coset_kv_cache* cache, const int64_t* slots, int64_t n, void* k, void* v, int dtype,
+                  void* stream);
+
+/* Attention of n new tokens of `seqs` sequences over the cache:
+ *   out[i, h] = sum_t softmax_t(scale q[i, h] . k_t) v_t
+ * over the tokens t that i sees, key head h / (heads / kv_heads), and lse[i, h]
+ * (nullable) = log sum_t exp(scale q[i, h] . k_t); a token that sees nothing
+ * gives zeros and -inf.  q [n, heads, head_dim] fp32, bf16 or fp16 (strides in
+ * elements), out contiguous in its type.
+ * starts: [seqs + 1] first new token of each sequence (int32), or NULL: n / seqs
+ * each.  lengths: [seqs] cached tokens of each sequence, its new ones the
+ * last.  block_table: [seqs, max_pages] pages of each sequence in order
+ * (int32, rows table_stride apart).  New token j of a sequence sees all
+ * cached tokens before the new ones and, of the new ones, those up to itself
+ * (tree_mask NULL) or those whose bit is set in its row of tree_mask
+ * [n, mask_words] (bit i % 64 of word i / 64: new token i of its sequence;
+ * tokens beyond the words are not seen).
+ * Lengths and pages outside the tables' bounds are clamped to them. */
+int64_t coset_kv_attention_workspace_floats(const coset_kv_cache* cache, int64_t n, int seqs, int heads, int dtype,
+                                            int64_t max_pages);
+int coset_kv_attention(const coset_kv_cache* cache, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                       int dtype, int64_t n, int heads, int seqs, const int32_t* starts, const int32_t* lengths,
+                       const int32_t* block_table, int64_t table_stride, int64_t max_pages, const int64_t* tree_mask,
+                       int64_t mask_words, float scale, void* out, float* lse, float* workspace,
+                       int64_t workspace_floats, void* stream);
+
+/* RMS norm of each head's query and key and the position rotation in one
+ * pass (no reference counterpart), for x = q [n, q_heads, dim] and k [n,
+ * k_heads, dim] in one type (strides in elements):
+ *   z = x (mean x^2 + eps)^(-1/2) w   (norm = 0: z = x)
+ *   (y_a, y_b) = (z_a cos - z_b sin, z_b cos + z_a sin) for the rot / 2 pairs,
+ * pair i being (i, i + rot/2) or, interleaved, (2i, 2i + 1); the other
+ * dim - rot values are z.  table: [length, rot] fp32, the pairs' cosines then
+ * their sines; pair i's row is positions[axis, token] (int64, clamped to the
+ * table, axes pos_stride apart), axis the first whose bounds[axis] is above i.
+ * w_q, w_k: [dim] in w_dtype, nullable (ones).  Outputs contiguous.  dim and
+ * rot are multiples of 8, dim <= 512, axes <= 4. */
+typedef struct coset_rope_side {
+    const void* x;
+    const void* grad;       /* backward: gradient of the output */
+    void* out;              /* output, or (backward) gradient of x */
+    const void* weight;
+    void* weight_grad;      /* backward, nullable */
+    int64_t token_stride, head_stride, grad_token_stride, grad_head_stride;
+    int64_t heads;
+} coset_rope_side;
+
+typedef struct coset_rope {
+    const float* table;
+    const int64_t* positions;
+    int64_t n, length, pos_stride;
+    int32_t dim, rot, axes, bounds[4];
+    int32_t norm, interleaved, dtype, w_dtype;
+    float eps;
+} coset_rope;
+
+int coset_qk_norm_rope_fwd(const coset_rope* r, const coset_rope_side* q, const coset_rope_side* k, void* stream);
+
+/* Its backward; the weights' gradients are summed in a fixed order through a
+ * workspace of coset_qk_norm_rope_workspace_floats (needed where either is
+ * asked for). */
+int64_t coset_qk_norm_rope_workspace_floats(int64_t n, int dim);
+int coset_qk_norm_rope_bwd(const coset_rope* r, const coset_rope_side* q, const coset_rope_side* k, float* workspace,
+                           int64_t workspace_floats, void* stream);
+
 /* Elementwise lattice operator over n_blocks fp32 blocks (custom_round is
  * applied to all 8*n_blocks values).  legacy selects the legacy g_x rule. */
 int coset_e8_lattice_op(int op, int legacy, const float* in, int64_t n_blocks, int q,
