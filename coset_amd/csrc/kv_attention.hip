@@ -51,8 +51,13 @@ constexpr int kStep = kTile * kWaves;       // tokens of a workgroup's step
 constexpr float kNone = -1e30f;             // M of a row that has seen nothing
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// log2 of a weight with respect to M: after a move, and where the next move is due
-constexpr float kSettle = 9.f, kDue = 14.f;
+// Tables that no kernel of the call writes, read through the scalar cache
+// where the index is the same in all lanes.
+typedef const __attribute__((address_space(4))) int32_t* ConstInts;
+__device__ __forceinline__ ConstInts constant(const int32_t* p) { return (ConstInts)(uintptr_t)p; }
+
+// log2 of the largest weight with respect to M after a move, and the weight at which the next move is due
+constexpr float kSettle = 9.f, kDue = 0x1p14f;
 
 // One descriptor a workgroup: the parts of the segment that begins in it and
 // goes on in the next ones (0: none).
@@ -80,14 +85,14 @@ __device__ __forceinline__ Seq seq_of(const KvAttentionArgs& a, int b)
     Seq s;
     if (a.starts) {
         // starts outside [0, n], or in falling order: no tokens
-        const int lo = a.starts[b], hi = a.starts[b + 1];
+        const int lo = constant(a.starts)[b], hi = constant(a.starts)[b + 1];
         s.token0 = min(max(lo, 0), (int)a.n);
         s.tokens = max(min(max(hi, 0), (int)a.n) - s.token0, 0);
     } else {
         s.tokens = (int)(a.n / a.seqs);
         s.token0 = b * s.tokens;
     }
-    s.length = min(max(a.lengths[b], 0), (int)min((int64_t)a.max_pages * a.c.page_size, (int64_t)0x7fffff00));
+    s.length = min(max(constant(a.lengths)[b], 0), (int)min((int64_t)a.max_pages * a.c.page_size, (int64_t)0x7fffff00));
     return s;
 }
 
@@ -126,12 +131,12 @@ template <int BITS, bool CENTER>
 __device__ __forceinline__ void key_operand(const uint32_t* w, uint32_t (&r)[4])
 {
     if constexpr (BITS == 4) {
-        const uint32_t base = 0x4c004c00u | ((uint32_t)((int32_t)(w[0] << 3) >> 31) & 0x00200020u);
-        const uint32_t u = w[0] ^ ((uint32_t)__popc(w[0] & 0x11111111u) << 31 >> 3);
-        r[0] = nibbles<0>(u, base);
-        r[1] = nibbles<1>(u, base);
-        r[2] = nibbles<2>(u, base);
-        r[3] = nibbles<3>(u, base);
+        const uint32_t base = ((uint32_t)__builtin_amdgcn_sbfe((int)w[0], 28, 1) & 0x00200020u) | 0x4c004c00u;
+        r[0] = nibbles<0>(w[0], base);
+        r[1] = nibbles<1>(w[0], base);
+        r[2] = nibbles<2>(w[0], base);
+        // n_7's lowest bit, at 22 here: h there, xor the parity of the word's lowest bits
+        r[3] = nibbles<3>(w[0], base) ^ ((uint32_t)__popc(w[0] & 0x11111111u) << 22 & 0x00400000u);
     } else {
         const uint32_t h = (w[1] >> 24) & 1u;
         const uint32_t base = 0x60006000u | h | (h << 16);
@@ -197,45 +202,65 @@ __device__ __forceinline__ void value_pair(const uint32_t* a, const uint32_t* b,
 }
 
 // What a wave loads for 16 tokens: a lane's blocks of one key, four tokens'
-// words of its block (or two blocks) of the values, four tokens' scales.
+// words of its block (or two blocks) of the values, four tokens' scales.  The
+// row is wave-uniform, a lane's place in it is fixed.
 template <int DP, int BITS>
 struct Words {
     static constexpr int W = BITS / 4;
     static constexpr int C = DP / 32;               // 32-coordinate chunks: a lane's blocks of a key
     static constexpr int B = DP == 256 ? 2 : 1;     // a lane's blocks of the values
-    uint32_t k[C * W];
-    uint32_t v[B][4 * W];
-    uint32_t sc[4];
+    static constexpr int KL = C * W == 2 ? 1 : C * W / 4;   // loads of a lane's keys
+    uint32_t k_at[KL], v_at[B], s_at;               // byte offsets from the row
+    int row_bytes;
 
-    __device__ __forceinline__ void load(const KvCache& c, int64_t row, int lane)
+    __device__ __forceinline__ void init(const KvCache& c, int lane)
     {
         const int nb = c.dim >> 3, g = lane >> 4, m = lane & 15;
-        const uint32_t* kp = c.k + (row + m) * (int64_t)(nb * W);
+        row_bytes = 4 * nb * W;
         if constexpr (C * W == 2) {
-            const uint2 u = *reinterpret_cast<const uint2*>(kp + 2 * min(g, nb / 2 - 1));
+            k_at[0] = m * row_bytes + 8 * min(g, nb / 2 - 1);
+        } else {
+#pragma unroll
+            for (int i = 0; i < KL; ++i) k_at[i] = m * row_bytes + 16 * min(g * KL + i, nb * W / 4 - 1);
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) v_at[b] = 4 * g * row_bytes + 16 * W * min(DP == 64 ? m & 7 : 16 * b + m, nb - 1);
+        s_at = 16 * g;
+    }
+
+    __device__ __forceinline__ void keys(const KvCache& c, int64_t row, uint32_t (&k)[C * W]) const
+    {
+        const char* p = reinterpret_cast<const char*>(c.k) + row * row_bytes;
+        if constexpr (C * W == 2) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p + k_at[0]);
             k[0] = u.x;
             k[1] = u.y;
         } else {
-            const int last = nb * W / 4 - 1;
 #pragma unroll
-            for (int i = 0; i < C * W / 4; ++i) {
-                const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(kp + 4 * min(g * (C * W / 4) + i, last));
+            for (int i = 0; i < KL; ++i) {
+                const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(p + k_at[i]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) k[4 * i + j] = u[j];
             }
         }
-        const uint32_t* vp = c.v + (row + 4 * g) * (int64_t)(nb * W);
+    }
+
+    __device__ __forceinline__ void values(const KvCache& c, int64_t row, uint32_t (&v)[B][4 * W]) const
+    {
+        const char* p = reinterpret_cast<const char*>(c.v) + row * row_bytes;
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
-            const int block = min(DP == 64 ? m & 7 : 16 * b + m, nb - 1);
+        for (int b = 0; b < B; ++b)
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(vp + 4 * W * block + 4 * i);
+                const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(p + v_at[b] + 16 * i);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[b][4 * i + j] = u[j];
             }
-        }
-        const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(c.scales + row + 4 * g);
+    }
+
+    __device__ __forceinline__ void scales(const KvCache& c, int64_t row, uint32_t (&sc)[4]) const
+    {
+        const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(reinterpret_cast<const char*>(c.scales) + row * 4 + s_at);
 #pragma unroll
         for (int j = 0; j < 4; ++j) sc[j] = u[j];
     }
@@ -253,6 +278,23 @@ __device__ __forceinline__ float over_groups_sum(float v)
     return v + __shfl_xor(v, 32, 64);
 }
 
+// Which of the tokens place .. place + 3 a row sees: those below its limit
+// and, with a mask, the drafted ones whose bits its row of the mask sets.
+__device__ __forceinline__ uint32_t seen_of(const KvAttentionArgs& a, const Seq& sq, int limit, int own, int place)
+{
+    uint32_t seen = 0;
+    const int ctx = sq.length - sq.tokens;
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+        const int at = place + i, d = at - ctx;
+        bool on = at < limit;
+        if (a.mask && !on && own >= 0 && at < sq.length && d >= 0 && d < 64 * a.mask_words)
+            on = (a.mask[(int64_t)own * a.mask_words + (d >> 6)] >> (d & 63)) & 1;
+        seen |= on ? 1u << i : 0u;
+    }
+    return seen;
+}
+
 template <int DT>
 __device__ __forceinline__ void load_query(const KvAttentionArgs& a, int64_t at, float (&x)[8])
 {
@@ -261,8 +303,8 @@ __device__ __forceinline__ void load_query(const KvAttentionArgs& a, int64_t at,
 
 // DP: dim padded to 64, 128 or 256; NR: 16-row tiles; QS: queries in two fp16
 // parts; PS: weights in two.
-template <int DP, int BITS, int NR, int DT, bool QS, bool PS>
-__global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs a, int most_parts)
+template <int DP, int BITS, int NR, int DT, bool QS, bool PS, int OCC>
+__global__ void __launch_bounds__(kThreads, OCC) kv_attention_kernel(KvAttentionArgs a, int most_parts)
 {
     using T = Words<DP, BITS>;
     constexpr int C = T::C, W = T::W;
@@ -273,8 +315,10 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs 
     __shared__ __align__(16) float sh_o[kWaves][16 * kPitch];
     __shared__ float sh_m[kWaves][kRows], sh_l[kWaves][kRows];
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
+    T words;
+    words.init(a.c, lane);
     // neighbouring runs on one XCD (workgroups go to the 8 XCDs in turn)
     const int id = (int)(blockIdx.x & 7) * (gridDim.x >> 3) + (int)(blockIdx.x >> 3);
 
@@ -286,6 +330,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs 
         for (int o = 1; o < 64; o <<= 1) u += __shfl_xor(u, o, 64);
         total += u;
     }
+    total = __builtin_amdgcn_readfirstlane(total);
     const int run = (total + (int)gridDim.x - 1) / (int)gridDim.x;
     int unit = id * run;
     const int end = min(unit + run, total);
@@ -355,8 +400,9 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs 
             top = over_groups_max(top);
             // times 2^k, which brings the row's largest value to [2^10, 2^11)
             const int e = max((int)(__float_as_uint(top) >> 23), 20);
-            const float up = __uint_as_float((uint32_t)(264 - e) << 23);
-            q_scale[r] = a.scale * __uint_as_float((uint32_t)(e - 10) << 23);
+            const float up = copysignf(__uint_as_float((uint32_t)(264 - e) << 23), a.scale);
+            // above zero, so that a hidden token's score stays at minus infinity
+            q_scale[r] = fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(e - 10) << 23), 0x1p-126f);
             float sum = 0.f;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
@@ -386,7 +432,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs 
         // tokens that any row of the tile may see, and those that all see
         const int reach = a.mask ? sq.length : min(sq.length, ctx + t_last + 1);
         const int all = a.mask ? ctx : ctx + t_first + 1;
-        const int32_t* pages = a.table + (int64_t)b * a.table_stride;
+        const ConstInts pages = constant(a.table + (int64_t)b * a.table_stride);
         auto row_of = [&](int token) -> int64_t {
             const uint32_t i = u32div((uint32_t)token, a.c.page_div);
             const uint32_t page = min((uint32_t)max(pages[min((int)i, a.max_pages - 1)], 0), a.c.pages - 1);
@@ -395,17 +441,25 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs 
 
         int token = (step * kWaves + wave) * kTile;
         const int stop = min((step + count) * kStep, reach);
-        T cur[2], next[2];
+        // one set of registers: the next keys are loaded behind the scores'
+        // product, the next values behind the second one, so that each has
+        // about half a step to arrive
+        uint32_t kw[2][C * W], vw[2][T::B][4 * W], sc[2][4];
+        int64_t at[2];
         if (token < stop) {
-            cur[0].load(a.c, row_of(token), lane);
-            cur[1].load(a.c, row_of(token + 16 < reach ? token + 16 : token), lane);
+            at[0] = row_of(token);
+            at[1] = row_of(token + 16 < reach ? token + 16 : token);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) words.keys(a.c, at[h], kw[h]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) words.scales(a.c, at[h], sc[h]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) words.values(a.c, at[h], vw[h]);
         }
         for (; token < stop; token += kStep) {
-            const int ahead = token + kStep;
-            if (ahead < stop) {
-                next[0].load(a.c, row_of(ahead), lane);
-                next[1].load(a.c, row_of(ahead + 16 < reach ? ahead + 16 : ahead), lane);
-            }
+            const int ahead = token + kStep < stop ? token + kStep : token;
+            at[0] = row_of(ahead);
+            at[1] = row_of(ahead + 16 < reach ? ahead + 16 : ahead);
             // scores
             f32x4_kv s[2][NR];
 #pragma unroll
@@ -415,7 +469,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs 
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     uint32_t k[4];
-                    key_operand<BITS, QS>(&cur[h].k[c * W], k);
+                    key_operand<BITS, QS>(&kw[h][c * W], k);
                     const half8_kv ka = __builtin_bit_cast(half8_kv, u32x4_kv{k[0], k[1], k[2], k[3]});
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
@@ -429,56 +483,71 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs 
                     }
                 }
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) words.keys(a.c, at[h], kw[h]);
             // weights
             const bool whole = token + kTile <= all;
+            float bk[8], bv[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t u = sc[i >> 2][i & 3];
+                bk[i] = __uint_as_float(u << 16);
+                // a zero vector's scale as 2^-70 (its points are zeros): no infinity times zero below
+                bv[i] = __uint_as_float(max(u & 0xffff0000u, 0x1c800000u));
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) words.scales(a.c, at[h], sc[h]);
             uint32_t p_hi[NR][4], p_lo[NR][4];
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                float t[8], bv[8], top = -INFINITY;
+                float u[8], w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) u[i] = s[i >> 2][r][i & 3] * bk[i];
+                uint32_t seen = 0xffu;
+                if (!whole) {
+                    seen = seen_of(a, sq, limit[r], own[r], token + 4 * g) | seen_of(a, sq, limit[r], own[r], token + 16 + 4 * g) << 4;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) u[i] = seen >> i & 1u ? u[i] : -INFINITY;
+                }
+                float sum = 0.f, top = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint32_t sc = cur[i >> 2].sc[i & 3];
-                    t[i] = s[i >> 2][r][i & 3] * (__uint_as_float(sc << 16) * q_scale[r]);
-                    bv[i] = __uint_as_float(sc & 0xffff0000u);
-                    if (!whole) {
-                        const int at = token + 16 * (i >> 2) + 4 * g + (i & 3);
-                        bool seen = at < limit[r];
-                        if (a.mask && !seen && at < sq.length && own[r] >= 0) {
-                            const int d = at - ctx;
-                            if (d >= 0 && d < 64 * a.mask_words)
-                                seen = (a.mask[(int64_t)own[r] * a.mask_words + (d >> 6)] >> (d & 63)) & 1;
-                        }
-                        if (!seen) {
-                            t[i] = -INFINITY;
-                            bv[i] = 0.f;
-                        }
-                    }
-                    // log2 of the value's scale + 127, to a tenth, from its bits; 60 for a zero
-                    const float lb = fmaxf((float)sc * 0x1p-23f, 60.f);
-                    top = fmaxf(top, t[i] + lb);
+                    const float p = __builtin_amdgcn_exp2f(fmaf(u[i], q_scale[r], -M[r]));
+                    sum += p;
+                    w[i] = p * bv[i];
                 }
-                if (__any(top > M[r] + (127.f + kDue))) {
-                    const float to = fmaxf(M[r], over_groups_max(top) - (127.f + kSettle));
-                    const float f = exp2f(M[r] - to);
+                if (!whole) {   // zero times a NaN scale
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] = seen >> i & 1u ? w[i] : 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, w[i]);
+                if (__any(top > kDue)) {
+                    float most = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) most = fmaxf(most, fmaf(u[i], q_scale[r], __builtin_amdgcn_logf(bv[i])));
+                    const float to = fmaxf(M[r], over_groups_max(most) - kSettle);
+                    const float f = __builtin_amdgcn_exp2f(M[r] - to);
                     M[r] = to;
                     l[r] *= f;
 #pragma unroll
                     for (int j = 0; j < NT; ++j) o[r][j] *= f;
-                }
-                float w[8];
+                    sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(t[i] - M[r]);
-                    l[r] += p;
-                    w[i] = p * bv[i];
+                    for (int i = 0; i < 8; ++i) {
+                        const float p = __builtin_amdgcn_exp2f(fmaf(u[i], q_scale[r], -to));
+                        sum += p;
+                        w[i] = seen >> i & 1u ? p * bv[i] : 0.f;
+                    }
                 }
+                l[r] += sum;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     p_hi[r][i] = pack2<DT_F16>(w[2 * i], w[2 * i + 1]);
                     if constexpr (PS) {
-                        float u, v;
-                        unpack2<DT_F16>(p_hi[r][i], u, v);
-                        p_lo[r][i] = pack2<DT_F16>(w[2 * i] - u, w[2 * i + 1] - v);
+                        float x, y;
+                        unpack2<DT_F16>(p_hi[r][i], x, y);
+                        p_lo[r][i] = pack2<DT_F16>(w[2 * i] - x, w[2 * i + 1] - y);
                     }
                 }
             }
@@ -488,8 +557,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs 
                 uint32_t v[4][E];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    value_pair<BITS, E>(&cur[i >> 1].v[blk][(i & 1) * 2 * W], &cur[i >> 1].v[blk][((i & 1) * 2 + 1) * W],
-                                        n >= 8, v[i]);
+                    value_pair<BITS, E>(&vw[i >> 1][blk][(i & 1) * 2 * W], &vw[i >> 1][blk][((i & 1) * 2 + 1) * W], n >= 8, v[i]);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const half8_kv va = __builtin_bit_cast(half8_kv, u32x4_kv{v[0][e], v[1][e], v[2][e], v[3][e]});
@@ -505,8 +573,8 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs 
                     }
                 }
             }
-            cur[0] = next[0];
-            cur[1] = next[1];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) words.values(a.c, at[h], vw[h]);
         }
 
         // the four waves' rows
@@ -526,7 +594,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs 
             float m = sh_m[0][16 * r + n];
 #pragma unroll
             for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sh_m[w][16 * r + n]);
-            const float f = exp2f(M[r] - m);
+            const float f = __builtin_amdgcn_exp2f(M[r] - m);
             float* mine = &sh_o[wave][n * kPitch];
             if constexpr (DP == 64) {
 #pragma unroll
@@ -557,7 +625,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_kernel(KvAttentionArgs 
             for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, sh_m[w][rr]);
             float ll = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) ll += sh_l[w][rr] * exp2f(sh_m[w][rr] - mm);
+            for (int w = 0; w < kWaves; ++w) ll += sh_l[w][rr] * __builtin_amdgcn_exp2f(sh_m[w][rr] - mm);
             if (rr < rows) {
                 const uint32_t t = u32div((uint32_t)(row0 + rr), a.group_div);
                 const int hq = kh * a.group + (row0 + rr - (int)t * a.group);
@@ -643,7 +711,7 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(KvAttentionArgs a, in
     float l = 0.f;
     for (int p = lot; p < d.parts; p += kParts) {
         const int64_t at = slot(p);
-        const float f = exp2f(part_ml[at * 2] - m);
+        const float f = __builtin_amdgcn_exp2f(part_ml[at * 2] - m);
         l += part_ml[at * 2 + 1] * f;
         if (4 * across < a.c.dim) o += *reinterpret_cast<const f32x4_kv*>(part_o + at * DP + 4 * across) * f;
     }
@@ -665,13 +733,17 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(KvAttentionArgs a, in
     if (a.lse && across == 0) a.lse[at] = some ? (m + log2f(l)) * (1.f / kLog2e) : -INFINITY;
 }
 
+// Waves a SIMD, and so workgroups a CU, that the registers leave room for.
+constexpr int waves_of(int pad_dim, int tiles) { return pad_dim == 256 || tiles == 4 ? 1 : tiles == 2 ? 2 : 3; }
+
 template <int DP, int BITS, int NR, int DT>
 hipError_t launch(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_t s)
 {
     constexpr bool QS = DT == DT_F32, PS = DT != DT_BF16;
+    constexpr int OCC = waves_of(DP, NR);
     const int64_t most_tokens = (int64_t)a.max_pages * a.c.page_size;
     const int most_parts = (int)((most_tokens + kStep - 1) / kStep);
-    hipLaunchKernelGGL((kv_attention_kernel<DP, BITS, NR, DT, QS, PS>), dim3(p.blocks), dim3(kThreads), 0, s, a, most_parts);
+    hipLaunchKernelGGL((kv_attention_kernel<DP, BITS, NR, DT, QS, PS, OCC>), dim3(p.blocks), dim3(kThreads), 0, s, a, most_parts);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || most_parts <= 1) return e;
     // rows of a tile that can be in use
@@ -721,7 +793,7 @@ KvAttentionPlan kv_attention_plan(int64_t n, int seqs, int heads, int kv_heads, 
     const int64_t tiles = (n * (heads / kv_heads) + 16 * p.tiles - 1) / (16 * p.tiles) + seqs;
     const int64_t steps = (max_tokens + kStep - 1) / kStep;
     const int64_t units = p.units = tiles * kv_heads * (steps > 0 ? steps : 1);
-    const int64_t fit = 256 * (p.pad_dim == 256 || p.tiles == 4 ? 2 : 4);
+    const int64_t fit = 256 * waves_of(p.pad_dim, p.tiles);
     p.blocks = (int)(units < fit ? (units + 7) / 8 * 8 : fit);
     if (p.blocks < 8) p.blocks = 8;
     const int64_t r = 16 * p.tiles;
