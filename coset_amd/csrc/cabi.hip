@@ -997,7 +997,7 @@ static int kv_attention_shape(const coset::KvCache& c, int64_t n, int heads, int
     if (max_pages > 0x7fffff00 / (int64_t)c.page_size || n > 0x7fffffff / heads)
         return fail(COSET_EUNSUPPORTED, "max_pages * page_size and n * heads must stay below 2^31");
     p = coset::kv_attention_plan(n, seqs, heads, (int)c.heads, c.dim, c.bits, dtype, max_pages * c.page_size);
-    if (p.units > (1 << 30)) return fail(COSET_EUNSUPPORTED, "more than 2^30 steps of 128 tokens in one call");
+    if (p.units > (1 << 30)) return fail(COSET_EUNSUPPORTED, "more than 2^30 steps of 32 to 128 tokens in one call");
     return COSET_OK;
 }
 

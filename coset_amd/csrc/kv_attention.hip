@@ -51,6 +51,21 @@ constexpr int kStep = kTile * kWaves;       // tokens of a workgroup's step
 constexpr float kNone = -1e30f;             // M of a row that has seen nothing
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// Tokens of a step of the many-rows kernel: two buffers of their operands fit LDS twice.
+constexpr int span_of(int pad_dim) { return pad_dim == 256 ? 32 : 64; }
+
+// Waves a SIMD, and so workgroups a CU, that the registers leave room for.
+constexpr int waves_of(int pad_dim, int tiles, bool many)
+{
+    return many ? (pad_dim == 256 && tiles == 2 ? 1 : 2) : pad_dim == 256 ? 1 : tiles == 2 ? 2 : 3;
+}
+
+// The most 16-row tiles a wave holds without spilling.
+constexpr int tiles_of(int pad_dim, int dtype, bool many)
+{
+    return dtype == DT_F32 && pad_dim == 256 ? 1 : many || pad_dim < 256 ? 2 : 1;
+}
+
 // Tables that no kernel of the call writes, read through the scalar cache
 // where the index is the same in all lanes.
 typedef const __attribute__((address_space(4))) int32_t* ConstInts;
@@ -71,7 +86,7 @@ struct Desc {
 };
 
 struct Work {
-    int steps;       // of 128 tokens in a segment
+    int steps;       // in a segment
     int tiles;       // row tiles
     int units;       // steps * tiles * key heads
 };
@@ -96,10 +111,11 @@ __device__ __forceinline__ Seq seq_of(const KvAttentionArgs& a, int b)
     return s;
 }
 
-__device__ __forceinline__ Work work_of(const KvAttentionArgs& a, const Seq& s, int rows)
+// span: tokens of a step
+__device__ __forceinline__ Work work_of(const KvAttentionArgs& a, const Seq& s, int rows, int span)
 {
     Work w;
-    w.steps = max((s.length + kStep - 1) / kStep, 1);
+    w.steps = max((s.length + span - 1) / span, 1);
     w.tiles = (s.tokens * a.group + rows - 1) / rows;
     w.units = w.steps * w.tiles * (int)a.c.heads;
     return w;
@@ -258,6 +274,34 @@ struct Words {
             }
     }
 
+    // Half `half` of a lane's key words (of HALVES) and its block of the values' half.
+    template <int CH, int HALVES>
+    __device__ __forceinline__ void part(const KvCache& c, int64_t row, int half, uint32_t (&k)[CH * W], uint32_t (&v)[4 * W]) const
+    {
+        if constexpr (HALVES == 1) {
+            uint32_t vv[B][4 * W];
+            keys(c, row, k);
+            values(c, row, vv);
+#pragma unroll
+            for (int j = 0; j < 4 * W; ++j) v[j] = vv[0][j];
+        } else {
+            const char* kp = reinterpret_cast<const char*>(c.k) + row * row_bytes;
+            const char* vp = reinterpret_cast<const char*>(c.v) + row * row_bytes;
+#pragma unroll
+            for (int i = 0; i < KL / HALVES; ++i) {
+                const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(kp + (half ? k_at[KL / HALVES + i] : k_at[i]));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) k[4 * i + j] = u[j];
+            }
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(vp + (half ? v_at[B - 1] : v_at[0]) + 16 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[4 * i + j] = u[j];
+            }
+        }
+    }
+
     __device__ __forceinline__ void scales(const KvCache& c, int64_t row, uint32_t (&sc)[4]) const
     {
         const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(reinterpret_cast<const char*>(c.scales) + row * 4 + s_at);
@@ -295,94 +339,28 @@ __device__ __forceinline__ uint32_t seen_of(const KvAttentionArgs& a, const Seq&
     return seen;
 }
 
-template <int DT>
-__device__ __forceinline__ void load_query(const KvAttentionArgs& a, int64_t at, float (&x)[8])
-{
-    load_n<DT, 8>(a.q, at, a.vec, x);
-}
+// A wave's query rows as the first product's B operand, and their softmax
+// state.  Row 16 r + n of the wave is lane n's (and n + 16's, ...).
+template <int DP, int BITS, int NR, int DT, bool QS, bool PS>
+struct Rows {
+    static constexpr int C = DP / 32, NT = DP / 16;
+    uint32_t q_hi[NR][C][4], q_lo[NR][QS ? C : 1][4];
+    float scale[NR], bias[NR];   // of the scores; what the keys' offset adds to them, negated
+    int limit[NR], own[NR];      // a row sees tokens below limit; own: its query token, -1 for none
+    float M[NR], l[NR];
+    f32x4_kv o[NR][NT];
 
-// DP: dim padded to 64, 128 or 256; NR: 16-row tiles; QS: queries in two fp16
-// parts; PS: weights in two.
-template <int DP, int BITS, int NR, int DT, bool QS, bool PS, int OCC>
-__global__ void __launch_bounds__(kThreads, OCC) kv_attention_kernel(KvAttentionArgs a, int most_parts)
-{
-    using T = Words<DP, BITS>;
-    constexpr int C = T::C, W = T::W;
-    constexpr int E = DP == 64 ? 4 : 8;          // a lane's coordinates of a value block
-    constexpr int NT = DP / 16;                  // accumulator tiles of a row tile
-    constexpr int kRows = 16 * NR;
-    constexpr int kPitch = DP + 4;
-    __shared__ __align__(16) float sh_o[kWaves][16 * kPitch];
-    __shared__ float sh_m[kWaves][kRows], sh_l[kWaves][kRows];
-
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = lane >> 4, n = lane & 15;
-    T words;
-    words.init(a.c, lane);
-    // neighbouring runs on one XCD (workgroups go to the 8 XCDs in turn)
-    const int id = (int)(blockIdx.x & 7) * (gridDim.x >> 3) + (int)(blockIdx.x >> 3);
-
-    // the line of units: its length, this workgroup's run and where it begins
-    int total = 0;
-    for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-        int u = b0 + lane < a.seqs ? work_of(a, seq_of(a, b0 + lane), kRows).units : 0;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) u += __shfl_xor(u, o, 64);
-        total += u;
-    }
-    total = __builtin_amdgcn_readfirstlane(total);
-    const int run = (total + (int)gridDim.x - 1) / (int)gridDim.x;
-    int unit = id * run;
-    const int end = min(unit + run, total);
-    Desc* descs = reinterpret_cast<Desc*>(a.workspace);
-    float* part_ml = a.workspace + (int64_t)gridDim.x * (sizeof(Desc) / 4);
-    float* part_o = part_ml + (int64_t)gridDim.x * 2 * kRows * 2;
-    if (most_parts > 1 && threadIdx.x == 0 && unit >= end) descs[id].parts = 0;
-    if (unit >= end) return;
-    int b = 0, before = 0;
-    for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-        const int u = b0 + lane < a.seqs ? work_of(a, seq_of(a, b0 + lane), kRows).units : 0;
-        int sum = u;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(sum, o, 64);
-            sum += lane >= o ? up : 0;
-        }
-        const uint64_t past = __ballot(before + sum > unit);
-        if (past) {
-            const int first = __ffsll((unsigned long long)past) - 1;
-            b = b0 + first;
-            before += __shfl(sum - u, first, 64);
-            break;
-        }
-        before += __shfl(sum, 63, 64);
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
-    before = __builtin_amdgcn_readfirstlane(before);
-    Seq sq = seq_of(a, b);
-    Work wk = work_of(a, sq, kRows);
-    int seg = (unit - before) / wk.steps, step = (unit - before) % wk.steps;
-    if (most_parts > 1 && threadIdx.x == 0) descs[id].parts = 0;
-    if (seg >= wk.tiles * (int)a.c.heads) return;   // starts that overlap so far that the line's length wrapped
-
-    while (unit < end) {
-        const int count = min(wk.steps - step, end - unit);
-        const int kh = seg / wk.tiles, tile = seg % wk.tiles;
-        const int row0 = tile * kRows, rows = min(sq.tokens * a.group - row0, kRows);
-        const int ctx = sq.length - sq.tokens;
-        const int t_first = u32div((uint32_t)row0, a.group_div);
-        const int t_last = u32div((uint32_t)(row0 + rows - 1), a.group_div);
-
-        // the query rows
-        uint32_t q_hi[NR][C][4], q_lo[NR][QS ? C : 1][4];
-        float q_scale[NR], q_bias[NR];
-        int limit[NR], own[NR];     // a row sees tokens below limit; own: its query token
+    // first: the wave's first row in the segment's (token, head of the group) rows
+    __device__ __forceinline__ void begin(const KvAttentionArgs& a, const Seq& sq, int kh, int first, int lane)
+    {
+        const int g = lane >> 4, n = lane & 15;
+        const int ctx = sq.length - sq.tokens, rows = sq.tokens * a.group;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            const int row = 16 * r + n;
+            const int row = first + 16 * r + n;
             const bool on = row < rows;
-            const uint32_t t = u32div((uint32_t)(row0 + row), a.group_div);
-            const int hq = kh * a.group + (row0 + row - (int)t * a.group);
+            const uint32_t t = u32div((uint32_t)row, a.group_div);
+            const int hq = kh * a.group + (row - (int)t * a.group);
             own[r] = on ? sq.token0 + (int)t : -1;
             limit[r] = on ? (a.mask ? ctx : min(sq.length, ctx + (int)t + 1)) : 0;
             float x[C][8];
@@ -393,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_attention_kernel(KvAttention
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[c][j] = 0.f;
                 if (on && block < (a.c.dim >> 3))
-                    load_query<DT>(a, (int64_t)own[r] * a.q_tok + hq * a.q_head + 8 * block, x[c]);
+                    load_n<DT, 8>(a.q, (int64_t)own[r] * a.q_tok + hq * a.q_head + 8 * block, a.vec, x[c]);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[c][j]));
             }
@@ -402,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_attention_kernel(KvAttention
             const int e = max((int)(__float_as_uint(top) >> 23), 20);
             const float up = copysignf(__uint_as_float((uint32_t)(264 - e) << 23), a.scale);
             // above zero, so that a hidden token's score stays at minus infinity
-            q_scale[r] = fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(e - 10) << 23), 0x1p-126f);
+            scale[r] = fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(e - 10) << 23), 0x1p-126f);
             float sum = 0.f;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
@@ -416,39 +394,289 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_attention_kernel(KvAttention
                     if constexpr (QS) q_lo[r][c][i] = pack2<DT_F16>(u - hu, v - hv);
                 }
             }
-            q_bias[r] = QS ? 0.f : -kOffset<BITS> * over_groups_sum(sum);
-        }
-
-        float M[NR], l[NR];
-        f32x4_kv o[NR][NT];
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
+            bias[r] = QS ? 0.f : -kOffset<BITS> * over_groups_sum(sum);
             M[r] = kNone;
             l[r] = 0.f;
 #pragma unroll
             for (int j = 0; j < NT; ++j) o[r][j] = f32x4_kv{0.f, 0.f, 0.f, 0.f};
         }
+    }
+
+    // s += the keys' chunk c times the rows
+    __device__ __forceinline__ void score(f32x4_kv (&s)[NR], u32x4_kv k, int c) const
+    {
+        const half8_kv ka = __builtin_bit_cast(half8_kv, k);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            s[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                ka, __builtin_bit_cast(half8_kv, u32x4_kv{q_hi[r][c][0], q_hi[r][c][1], q_hi[r][c][2], q_hi[r][c][3]}),
+                s[r], 0, 0, 0);
+            if constexpr (QS)
+                s[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    ka, __builtin_bit_cast(half8_kv, u32x4_kv{q_lo[r][c][0], q_lo[r][c][1], q_lo[r][c][2], q_lo[r][c][3]}),
+                    s[r], 0, 0, 0);
+        }
+    }
+
+    // The weights of 32 tokens from their scores s and scale words sc, as the
+    // second product's B operand.  whole: every row sees all of them.
+    __device__ __forceinline__ void weigh(const KvAttentionArgs& a, const Seq& sq, const f32x4_kv (&s)[2][NR],
+                                          const uint32_t (&sc)[2][4], int token, bool whole, int g,
+                                          uint32_t (&p_hi)[NR][4], uint32_t (&p_lo)[NR][4])
+    {
+        float bk[8], bv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t u = sc[i >> 2][i & 3];
+            bk[i] = __uint_as_float(u << 16);
+            // a zero vector's scale as 2^-70 (its points are zeros): no infinity times zero below
+            bv[i] = __uint_as_float(max(u & 0xffff0000u, 0x1c800000u));
+        }
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            float u[8], w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = s[i >> 2][r][i & 3] * bk[i];
+            uint32_t seen = 0xffu;
+            if (!whole) {
+                seen = seen_of(a, sq, limit[r], own[r], token + 4 * g) | seen_of(a, sq, limit[r], own[r], token + 16 + 4 * g) << 4;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) u[i] = seen >> i & 1u ? u[i] : -INFINITY;
+            }
+            float sum = 0.f, top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(u[i], scale[r], -M[r]));
+                sum += p;
+                w[i] = p * bv[i];
+            }
+            if (!whole) {   // zero times a NaN scale
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = seen >> i & 1u ? w[i] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, w[i]);
+            if (__any(top > kDue)) {
+                float most = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) most = fmaxf(most, fmaf(u[i], scale[r], __builtin_amdgcn_logf(bv[i])));
+                const float to = fmaxf(M[r], over_groups_max(most) - kSettle);
+                const float f = __builtin_amdgcn_exp2f(M[r] - to);
+                M[r] = to;
+                l[r] *= f;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) o[r][j] *= f;
+                sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(u[i], scale[r], -to));
+                    sum += p;
+                    w[i] = seen >> i & 1u ? p * bv[i] : 0.f;
+                }
+            }
+            l[r] += sum;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p_hi[r][i] = pack2<DT_F16>(w[2 * i], w[2 * i + 1]);
+                if constexpr (PS) {
+                    float x, y;
+                    unpack2<DT_F16>(p_hi[r][i], x, y);
+                    p_lo[r][i] = pack2<DT_F16>(w[2 * i] - x, w[2 * i + 1] - y);
+                }
+            }
+        }
+    }
+
+    // accumulator tile j += the values' operand times the weights
+    __device__ __forceinline__ void add(u32x4_kv v, int j, const uint32_t (&p_hi)[NR][4], const uint32_t (&p_lo)[NR][4])
+    {
+        const half8_kv va = __builtin_bit_cast(half8_kv, v);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            o[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                va, __builtin_bit_cast(half8_kv, u32x4_kv{p_hi[r][0], p_hi[r][1], p_hi[r][2], p_hi[r][3]}), o[r][j], 0, 0, 0);
+            if constexpr (PS)
+                o[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    va, __builtin_bit_cast(half8_kv, u32x4_kv{p_lo[r][0], p_lo[r][1], p_lo[r][2], p_lo[r][3]}), o[r][j], 0, 0, 0);
+        }
+    }
+
+    // the first of 4 neighbouring dims that registers piece(i, q, ...) of a lane hold: i = 0..3, q = 0 .. DP / 64 - 1
+    __device__ __forceinline__ static int place(int i, int q, int g)
+    {
+        if constexpr (DP == 64) return 8 * ((4 * g + i) & 7) + 4 * (g >> 1);
+        return 128 * (q >> 1) + 8 * (4 * g + i) + 4 * (q & 1);
+    }
+    __device__ __forceinline__ f32x4_kv piece(int r, int i, int q) const
+    {
+        return f32x4_kv{o[r][4 * q][i], o[r][4 * q + 1][i], o[r][4 * q + 2][i], o[r][4 * q + 3][i]};
+    }
+};
+
+// A workgroup's run of the line of units.
+struct Line {
+    int unit, end, run;
+    int b, seg, step;   // where it begins: sequence, its segment, the segment's step
+    Seq sq;
+    Work wk;
+
+    // false: nothing to do
+    __device__ __forceinline__ bool begin(const KvAttentionArgs& a, int id, int blocks, int rows, int span, int lane)
+    {
+        int total = 0;
+        for (int b0 = 0; b0 < a.seqs; b0 += 64) {
+            int u = b0 + lane < a.seqs ? work_of(a, seq_of(a, b0 + lane), rows, span).units : 0;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) u += __shfl_xor(u, o, 64);
+            total += u;
+        }
+        total = __builtin_amdgcn_readfirstlane(total);
+        run = (total + blocks - 1) / blocks;
+        unit = id * run;
+        end = min(unit + run, total);
+        if (unit >= end) return false;
+        int at = 0, before = 0;
+        for (int b0 = 0; b0 < a.seqs; b0 += 64) {
+            const int u = b0 + lane < a.seqs ? work_of(a, seq_of(a, b0 + lane), rows, span).units : 0;
+            int sum = u;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int up = __shfl_up(sum, o, 64);
+                sum += lane >= o ? up : 0;
+            }
+            const uint64_t past = __ballot(before + sum > unit);
+            if (past) {
+                const int first = __ffsll((unsigned long long)past) - 1;
+                at = b0 + first;
+                before += __shfl(sum - u, first, 64);
+                break;
+            }
+            before += __shfl(sum, 63, 64);
+        }
+        b = __builtin_amdgcn_readfirstlane(at);
+        before = __builtin_amdgcn_readfirstlane(before);
+        sq = seq_of(a, b);
+        wk = work_of(a, sq, rows, span);
+        seg = (unit - before) / wk.steps;
+        step = (unit - before) % wk.steps;
+        // past the sequence: starts that overlap so far that the line's length wrapped
+        return seg < wk.tiles * (int)a.c.heads;
+    }
+
+    // behind `count` steps of the segment; false at the run's end
+    __device__ __forceinline__ bool next(const KvAttentionArgs& a, int count, int rows, int span)
+    {
+        unit += count;
+        step = 0;
+        if (unit >= end) return false;
+        if (++seg == wk.tiles * (int)a.c.heads) {
+            seg = 0;
+            do {
+                if (++b >= a.seqs) return false;
+                sq = seq_of(a, b);
+                wk = work_of(a, sq, rows, span);
+            } while (wk.units == 0);
+        }
+        return true;
+    }
+};
+
+// The workspace: descriptors, then each part's (M, l) and rows.  A workgroup
+// leaves at most two parts: of the segment it enters (slot 2 id) and of the
+// one it leaves unfinished (slot 2 id + 1).
+struct Parts {
+    Desc* descs;
+    float* ml;
+    float* o;
+    __device__ __forceinline__ Parts(float* ws, int blocks, int rows)
+    {
+        descs = reinterpret_cast<Desc*>(ws);
+        ml = ws + (int64_t)blocks * (sizeof(Desc) / 4);
+        o = ml + (int64_t)blocks * 2 * rows * 2;
+    }
+};
+
+__device__ __forceinline__ void leave(const Parts& parts, const KvAttentionArgs& a, const Line& ln, int id, int kh, int row0, int rows, int count)
+{
+    Desc d{};
+    d.parts = min(1 + (ln.wk.steps - count + ln.run - 1) / ln.run, (int)gridDim.x - id);
+    d.row0 = row0;
+    d.rows = rows;
+    d.token0 = ln.sq.token0;
+    d.head = kh;
+    parts.descs[id] = d;
+}
+
+// The cache row of a token (a multiple of 16) of sequence b's key head kh.
+struct Pages {
+    ConstInts table;
+    int kh;
+    __device__ __forceinline__ Pages(const KvAttentionArgs& a, int b, int kh_) : table(constant(a.table + (int64_t)b * a.table_stride)), kh(kh_) {}
+    __device__ __forceinline__ int64_t row(const KvAttentionArgs& a, int token) const
+    {
+        const uint32_t i = u32div((uint32_t)token, a.c.page_div);
+        const uint32_t page = min((uint32_t)max(table[min((int)i, a.max_pages - 1)], 0), a.c.pages - 1);
+        return ((int64_t)page * a.c.heads + kh) * a.c.page_size + (token - i * a.c.page_size);
+    }
+};
+
+__device__ __forceinline__ int xcd_id()
+{
+    // neighbouring runs on one XCD (workgroups go to the 8 XCDs in turn)
+    return (int)(blockIdx.x & 7) * (gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+}
+
+// Up to 32 rows: every wave holds all of them and takes 32 tokens of each
+// step, decoding words straight into operands.
+// DP: dim padded to 64, 128 or 256; NR: 16-row tiles; QS: queries in two fp16
+// parts; PS: weights in two; OCC: waves a SIMD.
+template <int DP, int BITS, int NR, int DT, bool QS, bool PS, int OCC>
+__global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a, int most_parts)
+{
+    using T = Words<DP, BITS>;
+    using R = Rows<DP, BITS, NR, DT, QS, PS>;
+    constexpr int C = T::C, W = T::W;
+    constexpr int E = DP == 64 ? 4 : 8;          // a lane's coordinates of a value block
+    constexpr int kRows = 16 * NR;
+    constexpr int kPitch = DP + 4;
+    __shared__ __align__(16) float sh_o[kWaves][16 * kPitch];
+    __shared__ float sh_m[kWaves][kRows], sh_l[kWaves][kRows];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const int id = xcd_id();
+    const Parts parts(a.workspace, (int)gridDim.x, kRows);
+    Line ln;
+    const bool some = ln.begin(a, id, (int)gridDim.x, kRows, kStep, lane);
+    if (most_parts > 1 && threadIdx.x == 0) parts.descs[id].parts = 0;
+    if (!some) return;
+    T words;
+    words.init(a.c, lane);
+
+    int count;
+    do {
+        const Seq& sq = ln.sq;
+        count = min(ln.wk.steps - ln.step, ln.end - ln.unit);
+        const int kh = ln.seg / ln.wk.tiles, tile = ln.seg % ln.wk.tiles;
+        const int row0 = tile * kRows, rows = min(sq.tokens * a.group - row0, kRows);
+        const int ctx = sq.length - sq.tokens;
+        R rs;
+        rs.begin(a, sq, kh, row0, lane);
 
         // tokens that any row of the tile may see, and those that all see
-        const int reach = a.mask ? sq.length : min(sq.length, ctx + t_last + 1);
-        const int all = a.mask ? ctx : ctx + t_first + 1;
-        const ConstInts pages = constant(a.table + (int64_t)b * a.table_stride);
-        auto row_of = [&](int token) -> int64_t {
-            const uint32_t i = u32div((uint32_t)token, a.c.page_div);
-            const uint32_t page = min((uint32_t)max(pages[min((int)i, a.max_pages - 1)], 0), a.c.pages - 1);
-            return ((int64_t)page * a.c.heads + kh) * a.c.page_size + (token - i * a.c.page_size);
-        };
-
-        int token = (step * kWaves + wave) * kTile;
-        const int stop = min((step + count) * kStep, reach);
+        const int reach = a.mask ? sq.length : min(sq.length, ctx + (int)u32div((uint32_t)(row0 + rows - 1), a.group_div) + 1);
+        const int all = a.mask ? ctx : ctx + (int)u32div((uint32_t)row0, a.group_div) + 1;
+        const Pages pages(a, ln.b, kh);
+        int token = (ln.step * kWaves + wave) * kTile;
+        const int stop = min((ln.step + count) * kStep, reach);
         // one set of registers: the next keys are loaded behind the scores'
         // product, the next values behind the second one, so that each has
         // about half a step to arrive
         uint32_t kw[2][C * W], vw[2][T::B][4 * W], sc[2][4];
         int64_t at[2];
         if (token < stop) {
-            at[0] = row_of(token);
-            at[1] = row_of(token + 16 < reach ? token + 16 : token);
+            at[0] = pages.row(a, token);
+            at[1] = pages.row(a, token + 16 < reach ? token + 16 : token);
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.keys(a.c, at[h], kw[h]);
 #pragma unroll
@@ -458,100 +686,26 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_attention_kernel(KvAttention
         }
         for (; token < stop; token += kStep) {
             const int ahead = token + kStep < stop ? token + kStep : token;
-            at[0] = row_of(ahead);
-            at[1] = row_of(ahead + 16 < reach ? ahead + 16 : ahead);
-            // scores
+            at[0] = pages.row(a, ahead);
+            at[1] = pages.row(a, ahead + 16 < reach ? ahead + 16 : ahead);
             f32x4_kv s[2][NR];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int r = 0; r < NR; ++r) s[h][r] = f32x4_kv{q_bias[r], q_bias[r], q_bias[r], q_bias[r]};
+                for (int r = 0; r < NR; ++r) s[h][r] = f32x4_kv{rs.bias[r], rs.bias[r], rs.bias[r], rs.bias[r]};
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     uint32_t k[4];
                     key_operand<BITS, QS>(&kw[h][c * W], k);
-                    const half8_kv ka = __builtin_bit_cast(half8_kv, u32x4_kv{k[0], k[1], k[2], k[3]});
-#pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        s[h][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            ka, __builtin_bit_cast(half8_kv, u32x4_kv{q_hi[r][c][0], q_hi[r][c][1], q_hi[r][c][2], q_hi[r][c][3]}),
-                            s[h][r], 0, 0, 0);
-                        if constexpr (QS)
-                            s[h][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                ka, __builtin_bit_cast(half8_kv, u32x4_kv{q_lo[r][c][0], q_lo[r][c][1], q_lo[r][c][2], q_lo[r][c][3]}),
-                                s[h][r], 0, 0, 0);
-                    }
+                    rs.score(s[h], u32x4_kv{k[0], k[1], k[2], k[3]}, c);
                 }
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.keys(a.c, at[h], kw[h]);
-            // weights
-            const bool whole = token + kTile <= all;
-            float bk[8], bv[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t u = sc[i >> 2][i & 3];
-                bk[i] = __uint_as_float(u << 16);
-                // a zero vector's scale as 2^-70 (its points are zeros): no infinity times zero below
-                bv[i] = __uint_as_float(max(u & 0xffff0000u, 0x1c800000u));
-            }
+            uint32_t p_hi[NR][4], p_lo[NR][4];
+            rs.weigh(a, sq, s, sc, token, token + kTile <= all, g, p_hi, p_lo);
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.scales(a.c, at[h], sc[h]);
-            uint32_t p_hi[NR][4], p_lo[NR][4];
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                float u[8], w[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) u[i] = s[i >> 2][r][i & 3] * bk[i];
-                uint32_t seen = 0xffu;
-                if (!whole) {
-                    seen = seen_of(a, sq, limit[r], own[r], token + 4 * g) | seen_of(a, sq, limit[r], own[r], token + 16 + 4 * g) << 4;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) u[i] = seen >> i & 1u ? u[i] : -INFINITY;
-                }
-                float sum = 0.f, top = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(u[i], q_scale[r], -M[r]));
-                    sum += p;
-                    w[i] = p * bv[i];
-                }
-                if (!whole) {   // zero times a NaN scale
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] = seen >> i & 1u ? w[i] : 0.f;
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, w[i]);
-                if (__any(top > kDue)) {
-                    float most = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) most = fmaxf(most, fmaf(u[i], q_scale[r], __builtin_amdgcn_logf(bv[i])));
-                    const float to = fmaxf(M[r], over_groups_max(most) - kSettle);
-                    const float f = __builtin_amdgcn_exp2f(M[r] - to);
-                    M[r] = to;
-                    l[r] *= f;
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) o[r][j] *= f;
-                    sum = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float p = __builtin_amdgcn_exp2f(fmaf(u[i], q_scale[r], -to));
-                        sum += p;
-                        w[i] = seen >> i & 1u ? p * bv[i] : 0.f;
-                    }
-                }
-                l[r] += sum;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p_hi[r][i] = pack2<DT_F16>(w[2 * i], w[2 * i + 1]);
-                    if constexpr (PS) {
-                        float x, y;
-                        unpack2<DT_F16>(p_hi[r][i], x, y);
-                        p_lo[r][i] = pack2<DT_F16>(w[2 * i] - x, w[2 * i + 1] - y);
-                    }
-                }
-            }
-            // values
 #pragma unroll
             for (int blk = 0; blk < T::B; ++blk) {
                 uint32_t v[4][E];
@@ -559,32 +713,20 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_attention_kernel(KvAttention
                 for (int i = 0; i < 4; ++i)
                     value_pair<BITS, E>(&vw[i >> 1][blk][(i & 1) * 2 * W], &vw[i >> 1][blk][((i & 1) * 2 + 1) * W], n >= 8, v[i]);
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const half8_kv va = __builtin_bit_cast(half8_kv, u32x4_kv{v[0][e], v[1][e], v[2][e], v[3][e]});
-#pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        o[r][blk * 8 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            va, __builtin_bit_cast(half8_kv, u32x4_kv{p_hi[r][0], p_hi[r][1], p_hi[r][2], p_hi[r][3]}),
-                            o[r][blk * 8 + e], 0, 0, 0);
-                        if constexpr (PS)
-                            o[r][blk * 8 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                va, __builtin_bit_cast(half8_kv, u32x4_kv{p_lo[r][0], p_lo[r][1], p_lo[r][2], p_lo[r][3]}),
-                                o[r][blk * 8 + e], 0, 0, 0);
-                    }
-                }
+                for (int e = 0; e < E; ++e) rs.add(u32x4_kv{v[0][e], v[1][e], v[2][e], v[3][e]}, blk * 8 + e, p_hi, p_lo);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.values(a.c, at[h], vw[h]);
         }
 
         // the four waves' rows
-        const bool done = count == wk.steps;
-        const int slot = 2 * id + (step == 0 ? 1 : 0);   // a segment's first part, or a later one
+        const bool done = count == ln.wk.steps;
+        const int64_t slot = 2 * id + (ln.step == 0 ? 1 : 0);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            const float sum = over_groups_sum(l[r]);
+            const float sum = over_groups_sum(rs.l[r]);
             if (g == 0) {
-                sh_m[wave][16 * r + n] = M[r];
+                sh_m[wave][16 * r + n] = rs.M[r];
                 sh_l[wave][16 * r + n] = sum;
             }
         }
@@ -594,28 +736,12 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_attention_kernel(KvAttention
             float m = sh_m[0][16 * r + n];
 #pragma unroll
             for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sh_m[w][16 * r + n]);
-            const float f = __builtin_amdgcn_exp2f(M[r] - m);
-            float* mine = &sh_o[wave][n * kPitch];
-            if constexpr (DP == 64) {
+            const float f = __builtin_amdgcn_exp2f(rs.M[r] - m);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = 8 * ((4 * g + i) & 7) + 4 * (g >> 1);
-                    *reinterpret_cast<f32x4_kv*>(mine + d) =
-                        f32x4_kv{o[r][0][i], o[r][1][i], o[r][2][i], o[r][3][i]} * f;
-                }
-            } else {
+            for (int q = 0; q < DP / 64; ++q)
 #pragma unroll
-                for (int blk = 0; blk < T::B; ++blk)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < 8; e += 4) {
-                            const int d = 128 * blk + 8 * (4 * g + i) + e;
-                            *reinterpret_cast<f32x4_kv*>(mine + d) =
-                                f32x4_kv{o[r][8 * blk + e][i], o[r][8 * blk + e + 1][i], o[r][8 * blk + e + 2][i],
-                                         o[r][8 * blk + e + 3][i]} * f;
-                        }
-            }
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4_kv*>(&sh_o[wave][n * kPitch + R::place(i, q, g)]) = rs.piece(r, i, q) * f;
             __syncthreads();
             // 16 rows x DP: a thread takes DP / 16 neighbours of one row in pieces of 8
             const int row = threadIdx.x >> 4;
@@ -647,58 +773,188 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_attention_kernel(KvAttention
                         for (int j = 0; j < 8; ++j) x[j] *= inv;
                         store_n<DT, 8>(a.out, at * a.c.dim + d, x);
                     } else {
-                        store_n<DT_F32, 8>(part_o, ((int64_t)slot * kRows + rr) * DP + d, x);
+                        store_n<DT_F32, 8>(parts.o, (slot * kRows + rr) * DP + d, x);
                     }
                 }
                 if ((threadIdx.x & 15) == 0) {
                     if (done) {
                         if (a.lse) a.lse[at] = ll > 0.f || ll != ll ? (mm + log2f(ll)) * (1.f / kLog2e) : -INFINITY;
                     } else {
-                        part_ml[((int64_t)slot * kRows + rr) * 2] = mm;
-                        part_ml[((int64_t)slot * kRows + rr) * 2 + 1] = ll;
+                        parts.ml[(slot * kRows + rr) * 2] = mm;
+                        parts.ml[(slot * kRows + rr) * 2 + 1] = ll;
                     }
                 }
             }
             __syncthreads();
         }
-        if (!done && step == 0 && threadIdx.x == 0) {
-            Desc d{};
-            d.parts = min(1 + (wk.steps - count + run - 1) / run, (int)gridDim.x - id);
-            d.row0 = row0;
-            d.rows = rows;
-            d.token0 = sq.token0;
-            d.head = kh;
-            descs[id] = d;
+        if (!done && ln.step == 0 && threadIdx.x == 0) leave(parts, a, ln, id, kh, row0, rows, count);
+    } while (ln.next(a, count, kRows, kStep));
+}
+
+// More rows: the four waves hold 16 * NR rows each and share the tokens,
+// which they decode once into operands in LDS, a quarter each: one buffer is
+// filled while the other one is used.
+template <int DP, int BITS, int NR, int DT, bool QS, bool PS, int OCC>
+__global__ void __launch_bounds__(kThreads, OCC) kv_many_kernel(KvAttentionArgs a, int most_parts)
+{
+    using T = Words<DP, BITS>;
+    using R = Rows<DP, BITS, NR, DT, QS, PS>;
+    constexpr int C = T::C, W = T::W, NT = R::NT;
+    constexpr int E = DP == 64 ? 4 : 8;
+    constexpr int kRows = 64 * NR;
+    constexpr int kSpan = span_of(DP);              // tokens of a step
+    constexpr int kSub = kSpan / 16;
+    constexpr int kHalves = 4 / kSub;               // a 16-token tile's keys and values go to 1 or 2 waves
+    constexpr int CH = C / kHalves;                 // key chunks a wave decodes
+    static_assert(T::B == kHalves, "one block of the values a lane");
+    __shared__ __align__(16) u32x4_kv sh_k[2][kSub][C][64];
+    __shared__ __align__(16) u32x4_kv sh_v[2][kSub / 2][NT][64];
+    __shared__ __align__(16) uint32_t sh_s[2][kSpan];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const int sub = wave % kSub, half = wave / kSub;
+    const int id = xcd_id();
+    const Parts parts(a.workspace, (int)gridDim.x, kRows);
+    Line ln;
+    const bool some = ln.begin(a, id, (int)gridDim.x, kRows, kSpan, lane);
+    if (most_parts > 1 && threadIdx.x == 0) parts.descs[id].parts = 0;
+    if (!some) return;
+    T words;
+    words.init(a.c, lane);
+
+    int count;
+    do {
+        const Seq& sq = ln.sq;
+        count = min(ln.wk.steps - ln.step, ln.end - ln.unit);
+        const int kh = ln.seg / ln.wk.tiles, tile = ln.seg % ln.wk.tiles;
+        const int row0 = tile * kRows, rows = min(sq.tokens * a.group - row0, kRows);
+        const int ctx = sq.length - sq.tokens;
+        // the wave's own rows
+        const int first = row0 + wave * 16 * NR, last = min(first + 16 * NR, row0 + rows) - 1;
+        R rs;
+        rs.begin(a, sq, kh, first, lane);
+        const int reach = a.mask ? sq.length : min(sq.length, ctx + (int)u32div((uint32_t)(row0 + rows - 1), a.group_div) + 1);
+        const int mine = last < first ? 0 : a.mask ? sq.length : min(sq.length, ctx + (int)u32div((uint32_t)last, a.group_div) + 1);
+        const int all = a.mask ? ctx : ctx + (int)u32div((uint32_t)first, a.group_div) + 1;
+        const Pages pages(a, ln.b, kh);
+        int token = ln.step * kSpan;
+        const int stop = min((ln.step + count) * kSpan, reach);
+
+        uint32_t kw[CH * W], vw[4 * W], sw;
+        auto fetch = [&](int from) {
+            const int t = from + 16 * sub;
+            const int64_t row = pages.row(a, t < reach ? t : from);
+            words.template part<CH, kHalves>(a.c, row, half, kw, vw);
+            sw = a.c.scales[row + n];
+        };
+        auto decode = [&](int buf) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                uint32_t k[4];
+                key_operand<BITS, QS>(&kw[c * W], k);
+                sh_k[buf][sub][half * CH + c][lane] = u32x4_kv{k[0], k[1], k[2], k[3]};
+            }
+            uint32_t v[2][E];
+            value_pair<BITS, E>(&vw[0], &vw[W], n >= 8, v[0]);
+            value_pair<BITS, E>(&vw[2 * W], &vw[3 * W], n >= 8, v[1]);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                reinterpret_cast<uint2*>(&sh_v[buf][sub >> 1][half * 8 + e][lane])[sub & 1] = make_uint2(v[0][e], v[1][e]);
+            if (half == 0 && lane < 16) sh_s[buf][16 * sub + lane] = sw;
+        };
+        if (token < stop) {
+            fetch(token);
+            decode(0);
+            if (token + kSpan < stop) fetch(token + kSpan);
+        }
+        __syncthreads();
+        for (int buf = 0; token < stop; token += kSpan, buf ^= 1) {
+#pragma unroll
+            for (int p = 0; p < kSub / 2; ++p) {
+                const int at = token + kTile * p;
+                if (at >= mine) break;
+                f32x4_kv s[2][NR];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) s[h][r] = f32x4_kv{rs.bias[r], rs.bias[r], rs.bias[r], rs.bias[r]};
+#pragma unroll
+                    for (int c = 0; c < C; ++c) rs.score(s[h], sh_k[buf][2 * p + h][c][lane], c);
+                }
+                uint32_t sc[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(&sh_s[buf][16 * (2 * p + h) + 4 * g]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sc[h][j] = u[j];
+                }
+                uint32_t p_hi[NR][4], p_lo[NR][4];
+                rs.weigh(a, sq, s, sc, at, at + kTile <= all, g, p_hi, p_lo);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) rs.add(sh_v[buf][p][j][lane], j, p_hi, p_lo);
+            }
+            if (token + kSpan < stop) {
+                decode(buf ^ 1);
+                if (token + 2 * kSpan < stop) fetch(token + 2 * kSpan);
+            }
+            __syncthreads();
         }
 
-        unit += count;
-        step = 0;
-        if (unit < end && ++seg == wk.tiles * (int)a.c.heads) {
-            seg = 0;
-            do {
-                if (++b >= a.seqs) return;
-                sq = seq_of(a, b);
-                wk = work_of(a, sq, kRows);
-            } while (wk.units == 0);
+        const bool done = count == ln.wk.steps;
+        const int64_t slot = 2 * id + (ln.step == 0 ? 1 : 0);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const float ll = over_groups_sum(rs.l[r]);
+            const int rr = first + 16 * r + n - row0;
+            if (rr < rows) {
+                const uint32_t t = u32div((uint32_t)(row0 + rr), a.group_div);
+                const int hq = kh * a.group + (row0 + rr - (int)t * a.group);
+                const int64_t at = ((int64_t)sq.token0 + t) * a.heads + hq;
+                const float f = done ? (ll > 0.f || ll != ll ? 1.f / ll : 0.f) : 1.f;
+#pragma unroll
+                for (int q = 0; q < DP / 64; ++q)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int d = R::place(i, q, g);
+                        if (d >= a.c.dim) continue;
+                        const f32x4_kv v = rs.piece(r, i, q) * f;
+                        const float x[4] = {v[0], v[1], v[2], v[3]};
+                        if (done)
+                            store_n<DT, 4>(a.out, at * a.c.dim + d, x);
+                        else
+                            store_n<DT_F32, 4>(parts.o, (slot * kRows + rr) * DP + d, x);
+                    }
+                if (g == 0) {
+                    if (done) {
+                        if (a.lse) a.lse[at] = ll > 0.f || ll != ll ? (rs.M[r] + log2f(ll)) * (1.f / kLog2e) : -INFINITY;
+                    } else {
+                        parts.ml[(slot * kRows + rr) * 2] = rs.M[r];
+                        parts.ml[(slot * kRows + rr) * 2 + 1] = ll;
+                    }
+                }
+            }
         }
-    }
+        if (!done && ln.step == 0 && threadIdx.x == 0) leave(parts, a, ln, id, kh, row0, rows, count);
+    } while (ln.next(a, count, kRows, kSpan));
 }
 
 // Joins the parts of the segment that begins in workgroup blockIdx.x: one
 // workgroup a row (blockIdx.y), DP / 4 threads across the row, the rest of
 // them across the parts.
-template <int DP, int NR, int DT>
+template <int DP, int ROWS, int DT>
 __global__ void __launch_bounds__(kThreads) kv_join_kernel(KvAttentionArgs a, int blocks)
 {
-    constexpr int kRows = 16 * NR;
+    constexpr int kRows = ROWS;
     constexpr int kAcross = DP / 4, kParts = kThreads / kAcross;
     __shared__ __align__(16) float sh_o[kParts][DP];
     __shared__ float sh_m[kParts], sh_l[kParts];
     const Desc d = reinterpret_cast<const Desc*>(a.workspace)[blockIdx.x];
     const int row = blockIdx.y;
     if (d.parts == 0 || row >= d.rows) return;
-    const float* part_ml = a.workspace + (int64_t)blocks * (sizeof(Desc) / 4);
-    const float* part_o = part_ml + (int64_t)blocks * 2 * kRows * 2;
+    const Parts parts(a.workspace, blocks, kRows);
+    const float* part_ml = parts.ml;
+    const float* part_o = parts.o;
     const int across = threadIdx.x % kAcross, lot = threadIdx.x / kAcross;
     auto slot = [&](int p) { return (int64_t)(2 * ((int)blockIdx.x + p) + (p == 0 ? 1 : 0)) * kRows + row; };
     float m = kNone;
@@ -733,22 +989,24 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(KvAttentionArgs a, in
     if (a.lse && across == 0) a.lse[at] = some ? (m + log2f(l)) * (1.f / kLog2e) : -INFINITY;
 }
 
-// Waves a SIMD, and so workgroups a CU, that the registers leave room for.
-constexpr int waves_of(int pad_dim, int tiles) { return pad_dim == 256 || tiles == 4 ? 1 : tiles == 2 ? 2 : 3; }
-
-template <int DP, int BITS, int NR, int DT>
+template <int DP, int BITS, int NR, int DT, bool MANY>
 hipError_t launch(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_t s)
 {
     constexpr bool QS = DT == DT_F32, PS = DT != DT_BF16;
-    constexpr int OCC = waves_of(DP, NR);
+    constexpr int OCC = waves_of(DP, NR, MANY);
+    constexpr int kRows = 16 * NR * (MANY ? kWaves : 1);
     const int64_t most_tokens = (int64_t)a.max_pages * a.c.page_size;
-    const int most_parts = (int)((most_tokens + kStep - 1) / kStep);
-    hipLaunchKernelGGL((kv_attention_kernel<DP, BITS, NR, DT, QS, PS, OCC>), dim3(p.blocks), dim3(kThreads), 0, s, a, most_parts);
+    const int span = MANY ? span_of(DP) : kStep;
+    const int most_parts = (int)((most_tokens + span - 1) / span);
+    if constexpr (MANY)
+        hipLaunchKernelGGL((kv_many_kernel<DP, BITS, NR, DT, QS, PS, OCC>), dim3(p.blocks), dim3(kThreads), 0, s, a, most_parts);
+    else
+        hipLaunchKernelGGL((kv_few_kernel<DP, BITS, NR, DT, QS, PS, OCC>), dim3(p.blocks), dim3(kThreads), 0, s, a, most_parts);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || most_parts <= 1) return e;
     // rows of a tile that can be in use
     const int64_t rows = a.starts ? a.n * a.group : a.n / a.seqs * a.group;
-    hipLaunchKernelGGL((kv_join_kernel<DP, NR, DT>), dim3(p.blocks, (unsigned)(rows < 16 * NR ? rows : 16 * NR)),
+    hipLaunchKernelGGL((kv_join_kernel<DP, kRows, DT>), dim3(p.blocks, (unsigned)(rows < kRows ? rows : kRows)),
                        dim3(kThreads), 0, s, a, p.blocks);
     return hipGetLastError();
 }
@@ -756,12 +1014,16 @@ hipError_t launch(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_
 template <int DP, int BITS, int DT>
 hipError_t by_tiles(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_t s)
 {
-    if (p.tiles == 1) return launch<DP, BITS, 1, DT>(a, p, s);
-    if constexpr (DT != DT_F32 || DP < 256) {
-        if (p.tiles == 2) return launch<DP, BITS, 2, DT>(a, p, s);
-    }
-    if constexpr (DT != DT_F32 && DP < 256) {
-        if (p.tiles == 4) return launch<DP, BITS, 4, DT>(a, p, s);
+    if (!p.many) {
+        if (p.tiles == 1) return launch<DP, BITS, 1, DT, false>(a, p, s);
+        if constexpr (tiles_of(DP, DT, false) >= 2) {
+            if (p.tiles == 2) return launch<DP, BITS, 2, DT, false>(a, p, s);
+        }
+    } else {
+        if (p.tiles == 1) return launch<DP, BITS, 1, DT, true>(a, p, s);
+        if constexpr (tiles_of(DP, DT, true) >= 2) {
+            if (p.tiles == 2) return launch<DP, BITS, 2, DT, true>(a, p, s);
+        }
     }
     return hipErrorInvalidValue;
 }
@@ -785,18 +1047,21 @@ KvAttentionPlan kv_attention_plan(int64_t n, int seqs, int heads, int kv_heads, 
     (void)bits;
     KvAttentionPlan p{};
     p.pad_dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-    const int64_t rows = (n + seqs - 1) / seqs * (heads / kv_heads);
-    const int most = dtype == DT_F32 ? (p.pad_dim == 256 ? 1 : 2) : (p.pad_dim == 256 ? 2 : 4);
-    p.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    const int64_t group = heads / kv_heads;
+    const int64_t rows = (n + seqs - 1) / seqs * group;   // of a sequence, on average
+    p.many = rows > 32;
+    p.tiles = p.many ? (rows > 64 ? 2 : 1) : (rows > 16 ? 2 : 1);
+    const int most = tiles_of(p.pad_dim, dtype, p.many);
     if (p.tiles > most) p.tiles = most;
+    const int64_t r = 16 * p.tiles * (p.many ? kWaves : 1);
+    const int span = p.many ? span_of(p.pad_dim) : kStep;
     // workgroups that fit the chip at once, fewer where the steps are fewer
-    const int64_t tiles = (n * (heads / kv_heads) + 16 * p.tiles - 1) / (16 * p.tiles) + seqs;
-    const int64_t steps = (max_tokens + kStep - 1) / kStep;
+    const int64_t tiles = (n * group + r - 1) / r + seqs;
+    const int64_t steps = (max_tokens + span - 1) / span;
     const int64_t units = p.units = tiles * kv_heads * (steps > 0 ? steps : 1);
-    const int64_t fit = 256 * waves_of(p.pad_dim, p.tiles);
+    const int64_t fit = 256 * waves_of(p.pad_dim, p.tiles, p.many);
     p.blocks = (int)(units < fit ? (units + 7) / 8 * 8 : fit);
     if (p.blocks < 8) p.blocks = 8;
-    const int64_t r = 16 * p.tiles;
     p.workspace_floats = (int64_t)p.blocks * ((int64_t)sizeof(Desc) / 4 + 2 * r * 2 + 2 * r * p.pad_dim);
     return p;
 }

@@ -33,13 +33,13 @@ struct KvAttentionArgs {
     float* workspace;
 };
 
-// How a call is cut: `rows` query rows (token x head of a group) per
-// workgroup, at most `blocks` workgroups.
+// How a call is cut.
 struct KvAttentionPlan {
-    int tiles;      // 16-row tiles a workgroup holds: 1, 2 or 4
+    bool many;      // the kernel whose waves share the tokens (else each has its own)
+    int tiles;      // 16-row tiles of query rows (token x head of a group) that a wave holds: 1 or 2
     int blocks;
     int pad_dim;    // 64, 128 or 256
-    int64_t units;  // steps of 128 tokens at most
+    int64_t units;  // steps at most
     int64_t workspace_floats;
 };
 KvAttentionPlan kv_attention_plan(int64_t n, int seqs, int heads, int kv_heads, int dim, int bits, int dtype,
