@@ -46,6 +46,7 @@ typedef uint32_t u32x4_kv __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
+constexpr int kManyWaves = 8;               // of the many-rows kernel
 constexpr int kTile = 32;                   // tokens of a wave's step
 constexpr int kStep = kTile * kWaves;       // tokens of a workgroup's step
 constexpr float kNone = -1e30f;             // M of a row that has seen nothing
@@ -54,16 +55,16 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // Tokens of a step of the many-rows kernel: two buffers of their operands fit LDS twice.
 constexpr int span_of(int pad_dim) { return pad_dim == 256 ? 32 : 64; }
 
-// Waves a SIMD, and so workgroups a CU, that the registers leave room for.
+// Waves a SIMD that the registers leave room for.
 constexpr int waves_of(int pad_dim, int tiles, bool many)
 {
-    return many ? (pad_dim == 256 && tiles == 2 ? 1 : 2) : pad_dim == 256 ? 1 : tiles == 2 ? 2 : 3;
+    return many ? (pad_dim == 256 || tiles == 2 ? 2 : 4) : pad_dim == 256 ? 1 : tiles == 2 ? 2 : 3;
 }
 
 // The most 16-row tiles a wave holds without spilling.
 constexpr int tiles_of(int pad_dim, int dtype, bool many)
 {
-    return dtype == DT_F32 && pad_dim == 256 ? 1 : many || pad_dim < 256 ? 2 : 1;
+    return pad_dim == 256 ? 1 : 2;
 }
 
 // Tables that no kernel of the call writes, read through the scalar cache
@@ -274,34 +275,6 @@ struct Words {
             }
     }
 
-    // Half `half` of a lane's key words (of HALVES) and its block of the values' half.
-    template <int CH, int HALVES>
-    __device__ __forceinline__ void part(const KvCache& c, int64_t row, int half, uint32_t (&k)[CH * W], uint32_t (&v)[4 * W]) const
-    {
-        if constexpr (HALVES == 1) {
-            uint32_t vv[B][4 * W];
-            keys(c, row, k);
-            values(c, row, vv);
-#pragma unroll
-            for (int j = 0; j < 4 * W; ++j) v[j] = vv[0][j];
-        } else {
-            const char* kp = reinterpret_cast<const char*>(c.k) + row * row_bytes;
-            const char* vp = reinterpret_cast<const char*>(c.v) + row * row_bytes;
-#pragma unroll
-            for (int i = 0; i < KL / HALVES; ++i) {
-                const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(kp + (half ? k_at[KL / HALVES + i] : k_at[i]));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) k[4 * i + j] = u[j];
-            }
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(vp + (half ? v_at[B - 1] : v_at[0]) + 16 * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[4 * i + j] = u[j];
-            }
-        }
-    }
-
     __device__ __forceinline__ void scales(const KvCache& c, int64_t row, uint32_t (&sc)[4]) const
     {
         const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(reinterpret_cast<const char*>(c.scales) + row * 4 + s_at);
@@ -322,19 +295,25 @@ __device__ __forceinline__ float over_groups_sum(float v)
     return v + __shfl_xor(v, 32, 64);
 }
 
+__device__ __forceinline__ uint32_t ones(int n) { return n <= 0 ? 0u : n >= 4 ? 15u : (1u << n) - 1u; }
+
 // Which of the tokens place .. place + 3 a row sees: those below its limit
-// and, with a mask, the drafted ones whose bits its row of the mask sets.
-__device__ __forceinline__ uint32_t seen_of(const KvAttentionArgs& a, const Seq& sq, int limit, int own, int place)
+// and, with a mask, the drafted ones whose bits its row of the mask sets
+// (first: the row's first word).
+__device__ __forceinline__ uint32_t seen_of(const KvAttentionArgs& a, const Seq& sq, int limit, int own, uint64_t first, int place)
 {
-    uint32_t seen = 0;
-    const int ctx = sq.length - sq.tokens;
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) {
-        const int at = place + i, d = at - ctx;
-        bool on = at < limit;
-        if (a.mask && !on && own >= 0 && at < sq.length && d >= 0 && d < 64 * a.mask_words)
-            on = (a.mask[(int64_t)own * a.mask_words + (d >> 6)] >> (d & 63)) & 1;
-        seen |= on ? 1u << i : 0u;
+    uint32_t seen = ones(limit - place);
+    if (a.mask) {
+        const int d = place - (sq.length - sq.tokens);
+        uint64_t bits = 0;
+        if (d > -4 && d < 64) bits = d < 0 ? first << -d : first >> d;
+        if (a.mask_words > 1 && d > 60 && own >= 0) {
+            const int64_t* row = a.mask + (int64_t)own * a.mask_words;
+            const int w = d >> 6, rest = d & 63;
+            bits = w < a.mask_words ? (uint64_t)row[w] >> rest : 0;
+            if (rest > 60 && w + 1 < a.mask_words) bits |= (uint64_t)row[w + 1] << (64 - rest);
+        }
+        seen |= (uint32_t)bits & ones(sq.length - place);
     }
     return seen;
 }
@@ -347,11 +326,14 @@ struct Rows {
     uint32_t q_hi[NR][C][4], q_lo[NR][QS ? C : 1][4];
     float scale[NR], bias[NR];   // of the scores; what the keys' offset adds to them, negated
     int limit[NR], own[NR];      // a row sees tokens below limit; own: its query token, -1 for none
+    uint64_t drafts[NR];         // its row of the mask, the first word
     float M[NR], l[NR];
     f32x4_kv o[NR][NT];
 
-    // first: the wave's first row in the segment's (token, head of the group) rows
-    __device__ __forceinline__ void begin(const KvAttentionArgs& a, const Seq& sq, int kh, int first, int lane)
+    // first: the wave's first row in the segment's (token, head of the group)
+    // rows; meanwhile: what may be loaded while the rows are on their way
+    template <class F>
+    __device__ __forceinline__ void begin(const KvAttentionArgs& a, const Seq& sq, int kh, int first, int lane, F meanwhile)
     {
         const int g = lane >> 4, n = lane & 15;
         const int ctx = sq.length - sq.tokens, rows = sq.tokens * a.group;
@@ -363,8 +345,8 @@ struct Rows {
             const int hq = kh * a.group + (row - (int)t * a.group);
             own[r] = on ? sq.token0 + (int)t : -1;
             limit[r] = on ? (a.mask ? ctx : min(sq.length, ctx + (int)t + 1)) : 0;
+            drafts[r] = a.mask && on ? (uint64_t)a.mask[(int64_t)own[r] * a.mask_words] : 0;
             float x[C][8];
-            float top = 0.f;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const int block = C * g + c;
@@ -372,9 +354,13 @@ struct Rows {
                 for (int j = 0; j < 8; ++j) x[c][j] = 0.f;
                 if (on && block < (a.c.dim >> 3))
                     load_n<DT, 8>(a.q, (int64_t)own[r] * a.q_tok + hq * a.q_head + 8 * block, a.vec, x[c]);
+            }
+            if (r == NR - 1) meanwhile();
+            float top = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[c][j]));
-            }
             top = over_groups_max(top);
             // times 2^k, which brings the row's largest value to [2^10, 2^11)
             const int e = max((int)(__float_as_uint(top) >> 23), 20);
@@ -439,7 +425,8 @@ struct Rows {
             for (int i = 0; i < 8; ++i) u[i] = s[i >> 2][r][i & 3] * bk[i];
             uint32_t seen = 0xffu;
             if (!whole) {
-                seen = seen_of(a, sq, limit[r], own[r], token + 4 * g) | seen_of(a, sq, limit[r], own[r], token + 16 + 4 * g) << 4;
+                seen = seen_of(a, sq, limit[r], own[r], drafts[r], token + 4 * g) |
+                       seen_of(a, sq, limit[r], own[r], drafts[r], token + 16 + 4 * g) << 4;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) u[i] = seen >> i & 1u ? u[i] : -INFINITY;
             }
@@ -513,6 +500,16 @@ struct Rows {
     }
 };
 
+__device__ __forceinline__ int over_lanes(int u, int lane)
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(u, o, 64);
+        u += lane >= o ? up : 0;
+    }
+    return u;
+}
+
 // A workgroup's run of the line of units.
 struct Line {
     int unit, end, run;
@@ -523,35 +520,31 @@ struct Line {
     // false: nothing to do
     __device__ __forceinline__ bool begin(const KvAttentionArgs& a, int id, int blocks, int rows, int span, int lane)
     {
-        int total = 0;
+        // inclusive sums over the sequences, 64 at a time; the last 64 stay for the search
+        int total = 0, u = 0, sum = 0;
         for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-            int u = b0 + lane < a.seqs ? work_of(a, seq_of(a, b0 + lane), rows, span).units : 0;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) u += __shfl_xor(u, o, 64);
-            total += u;
+            u = b0 + lane < a.seqs ? work_of(a, seq_of(a, b0 + lane), rows, span).units : 0;
+            sum = over_lanes(u, lane);
+            total += __builtin_amdgcn_readlane(sum, 63);
         }
-        total = __builtin_amdgcn_readfirstlane(total);
         run = (total + blocks - 1) / blocks;
         unit = id * run;
         end = min(unit + run, total);
         if (unit >= end) return false;
         int at = 0, before = 0;
         for (int b0 = 0; b0 < a.seqs; b0 += 64) {
-            const int u = b0 + lane < a.seqs ? work_of(a, seq_of(a, b0 + lane), rows, span).units : 0;
-            int sum = u;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int up = __shfl_up(sum, o, 64);
-                sum += lane >= o ? up : 0;
+            if (a.seqs > 64) {
+                u = b0 + lane < a.seqs ? work_of(a, seq_of(a, b0 + lane), rows, span).units : 0;
+                sum = over_lanes(u, lane);
             }
             const uint64_t past = __ballot(before + sum > unit);
             if (past) {
                 const int first = __ffsll((unsigned long long)past) - 1;
                 at = b0 + first;
-                before += __shfl(sum - u, first, 64);
+                before += __builtin_amdgcn_readlane(sum - u, first);
                 break;
             }
-            before += __shfl(sum, 63, 64);
+            before += __builtin_amdgcn_readlane(sum, 63);
         }
         b = __builtin_amdgcn_readfirstlane(at);
         before = __builtin_amdgcn_readfirstlane(before);
@@ -660,9 +653,6 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
         const int kh = ln.seg / ln.wk.tiles, tile = ln.seg % ln.wk.tiles;
         const int row0 = tile * kRows, rows = min(sq.tokens * a.group - row0, kRows);
         const int ctx = sq.length - sq.tokens;
-        R rs;
-        rs.begin(a, sq, kh, row0, lane);
-
         // tokens that any row of the tile may see, and those that all see
         const int reach = a.mask ? sq.length : min(sq.length, ctx + (int)u32div((uint32_t)(row0 + rows - 1), a.group_div) + 1);
         const int all = a.mask ? ctx : ctx + (int)u32div((uint32_t)row0, a.group_div) + 1;
@@ -674,7 +664,9 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
         // about half a step to arrive
         uint32_t kw[2][C * W], vw[2][T::B][4 * W], sc[2][4];
         int64_t at[2];
-        if (token < stop) {
+        R rs;
+        rs.begin(a, sq, kh, row0, lane, [&]() {
+            if (token >= stop) return;
             at[0] = pages.row(a, token);
             at[1] = pages.row(a, token + 16 < reach ? token + 16 : token);
 #pragma unroll
@@ -683,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
             for (int h = 0; h < 2; ++h) words.scales(a.c, at[h], sc[h]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.values(a.c, at[h], vw[h]);
-        }
+        });
         for (; token < stop; token += kStep) {
             const int ahead = token + kStep < stop ? token + kStep : token;
             at[0] = pages.row(a, ahead);
@@ -791,37 +783,44 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
     } while (ln.next(a, count, kRows, kStep));
 }
 
-// More rows: the four waves hold 16 * NR rows each and share the tokens,
-// which they decode once into operands in LDS, a quarter each: one buffer is
-// filled while the other one is used.
+// More rows: eight waves hold 16 * NR rows each and share the tokens, which
+// they decode once into operands in LDS, an eighth each: one buffer is filled
+// while the other one is used.
 template <int DP, int BITS, int NR, int DT, bool QS, bool PS, int OCC>
-__global__ void __launch_bounds__(kThreads, OCC) kv_many_kernel(KvAttentionArgs a, int most_parts)
+__global__ void __launch_bounds__(64 * kManyWaves, OCC) kv_many_kernel(KvAttentionArgs a, int most_parts)
 {
-    using T = Words<DP, BITS>;
     using R = Rows<DP, BITS, NR, DT, QS, PS>;
-    constexpr int C = T::C, W = T::W, NT = R::NT;
-    constexpr int E = DP == 64 ? 4 : 8;
-    constexpr int kRows = 64 * NR;
+    constexpr int C = R::C, NT = R::NT, W = BITS / 4;
+    constexpr int kRows = 16 * NR * kManyWaves;
     constexpr int kSpan = span_of(DP);              // tokens of a step
     constexpr int kSub = kSpan / 16;
-    constexpr int kHalves = 4 / kSub;               // a 16-token tile's keys and values go to 1 or 2 waves
-    constexpr int CH = C / kHalves;                 // key chunks a wave decodes
-    static_assert(T::B == kHalves, "one block of the values a lane");
+    constexpr int kPieces = kManyWaves / kSub;      // waves that share 16 tokens' keys and values
+    static_assert(DP == 64 ? kPieces == 2 : C == 2 * kPieces, "two key chunks a wave");
     __shared__ __align__(16) u32x4_kv sh_k[2][kSub][C][64];
     __shared__ __align__(16) u32x4_kv sh_v[2][kSub / 2][NT][64];
     __shared__ __align__(16) uint32_t sh_s[2][kSpan];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
-    const int sub = wave % kSub, half = wave / kSub;
+    const int sub = wave % kSub, piece = wave / kSub;
     const int id = xcd_id();
     const Parts parts(a.workspace, (int)gridDim.x, kRows);
     Line ln;
     const bool some = ln.begin(a, id, (int)gridDim.x, kRows, kSpan, lane);
     if (most_parts > 1 && threadIdx.x == 0) parts.descs[id].parts = 0;
     if (!some) return;
-    T words;
-    words.init(a.c, lane);
+
+    // A wave's piece of 16 tokens: two chunks of the keys (DP = 64: piece 0
+    // takes both, piece 1 the values) and four coordinates of a block of the
+    // values, upper or lower.
+    const bool has_keys = DP > 64 || piece == 0, has_values = DP > 64 || piece == 1;
+    const int nb = a.c.dim >> 3, row_bytes = 4 * nb * W;
+    const int chunk = DP > 64 ? 2 * piece : 0;
+    const uint32_t k_at = n * row_bytes + 4 * W * min(C * g + chunk, nb - 2);
+    const int blk = DP == 256 ? piece >> 1 : 0;
+    const uint32_t v_at = 4 * g * row_bytes + 16 * W * min(DP == 64 ? n & 7 : 16 * blk + n, nb - 1);
+    const bool upper = DP == 64 ? n >= 8 : piece & 1;
+    const int v_tile = DP == 64 ? 0 : 8 * blk + 4 * (piece & 1);
 
     int count;
     do {
@@ -832,8 +831,6 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_many_kernel(KvAttentionArgs 
         const int ctx = sq.length - sq.tokens;
         // the wave's own rows
         const int first = row0 + wave * 16 * NR, last = min(first + 16 * NR, row0 + rows) - 1;
-        R rs;
-        rs.begin(a, sq, kh, first, lane);
         const int reach = a.mask ? sq.length : min(sq.length, ctx + (int)u32div((uint32_t)(row0 + rows - 1), a.group_div) + 1);
         const int mine = last < first ? 0 : a.mask ? sq.length : min(sq.length, ctx + (int)u32div((uint32_t)last, a.group_div) + 1);
         const int all = a.mask ? ctx : ctx + (int)u32div((uint32_t)first, a.group_div) + 1;
@@ -841,30 +838,57 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_many_kernel(KvAttentionArgs 
         int token = ln.step * kSpan;
         const int stop = min((ln.step + count) * kSpan, reach);
 
-        uint32_t kw[CH * W], vw[4 * W], sw;
+        uint32_t kw[2 * W], vw[4 * W], sw;
         auto fetch = [&](int from) {
             const int t = from + 16 * sub;
             const int64_t row = pages.row(a, t < reach ? t : from);
-            words.template part<CH, kHalves>(a.c, row, half, kw, vw);
-            sw = a.c.scales[row + n];
+            if (has_keys) {
+                const char* p = reinterpret_cast<const char*>(a.c.k) + row * row_bytes + k_at;
+                if constexpr (W == 1) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(p);
+                    kw[0] = u.x;
+                    kw[1] = u.y;
+                } else {
+                    const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(p);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) kw[j] = u[j];
+                }
+            }
+            if (has_values) {
+                const char* p = reinterpret_cast<const char*>(a.c.v) + row * row_bytes + v_at;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(p + 16 * i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) vw[4 * i + j] = u[j];
+                }
+            }
+            if (piece == 0) sw = a.c.scales[row + n];
         };
         auto decode = [&](int buf) {
+            if (has_keys) {
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                uint32_t k[4];
-                key_operand<BITS, QS>(&kw[c * W], k);
-                sh_k[buf][sub][half * CH + c][lane] = u32x4_kv{k[0], k[1], k[2], k[3]};
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t k[4];
+                    key_operand<BITS, QS>(&kw[c * W], k);
+                    sh_k[buf][sub][chunk + c][lane] = u32x4_kv{k[0], k[1], k[2], k[3]};
+                }
             }
-            uint32_t v[2][E];
-            value_pair<BITS, E>(&vw[0], &vw[W], n >= 8, v[0]);
-            value_pair<BITS, E>(&vw[2 * W], &vw[3 * W], n >= 8, v[1]);
+            if (has_values) {
+                uint32_t v[2][4];
+                value_pair<BITS, 4>(&vw[0], &vw[W], upper, v[0]);
+                value_pair<BITS, 4>(&vw[2 * W], &vw[3 * W], upper, v[1]);
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                reinterpret_cast<uint2*>(&sh_v[buf][sub >> 1][half * 8 + e][lane])[sub & 1] = make_uint2(v[0][e], v[1][e]);
-            if (half == 0 && lane < 16) sh_s[buf][16 * sub + lane] = sw;
+                for (int e = 0; e < 4; ++e)
+                    reinterpret_cast<uint2*>(&sh_v[buf][sub >> 1][v_tile + e][lane])[sub & 1] = make_uint2(v[0][e], v[1][e]);
+            }
+            if (piece == 0 && lane < 16) sh_s[buf][16 * sub + lane] = sw;
         };
+        R rs;
+        rs.begin(a, sq, kh, first, lane, [&]() {
+            if (token < stop) fetch(token);
+        });
         if (token < stop) {
-            fetch(token);
             decode(0);
             if (token + kSpan < stop) fetch(token + kSpan);
         }
@@ -994,12 +1018,12 @@ hipError_t launch(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_
 {
     constexpr bool QS = DT == DT_F32, PS = DT != DT_BF16;
     constexpr int OCC = waves_of(DP, NR, MANY);
-    constexpr int kRows = 16 * NR * (MANY ? kWaves : 1);
+    constexpr int kRows = 16 * NR * (MANY ? kManyWaves : 1);
     const int64_t most_tokens = (int64_t)a.max_pages * a.c.page_size;
     const int span = MANY ? span_of(DP) : kStep;
     const int most_parts = (int)((most_tokens + span - 1) / span);
     if constexpr (MANY)
-        hipLaunchKernelGGL((kv_many_kernel<DP, BITS, NR, DT, QS, PS, OCC>), dim3(p.blocks), dim3(kThreads), 0, s, a, most_parts);
+        hipLaunchKernelGGL((kv_many_kernel<DP, BITS, NR, DT, QS, PS, OCC>), dim3(p.blocks), dim3(64 * kManyWaves), 0, s, a, most_parts);
     else
         hipLaunchKernelGGL((kv_few_kernel<DP, BITS, NR, DT, QS, PS, OCC>), dim3(p.blocks), dim3(kThreads), 0, s, a, most_parts);
     hipError_t e = hipGetLastError();
@@ -1050,16 +1074,16 @@ KvAttentionPlan kv_attention_plan(int64_t n, int seqs, int heads, int kv_heads, 
     const int64_t group = heads / kv_heads;
     const int64_t rows = (n + seqs - 1) / seqs * group;   // of a sequence, on average
     p.many = rows > 32;
-    p.tiles = p.many ? (rows > 64 ? 2 : 1) : (rows > 16 ? 2 : 1);
+    p.tiles = p.many ? (rows > 128 ? 2 : 1) : (rows > 16 ? 2 : 1);
     const int most = tiles_of(p.pad_dim, dtype, p.many);
     if (p.tiles > most) p.tiles = most;
-    const int64_t r = 16 * p.tiles * (p.many ? kWaves : 1);
+    const int64_t r = 16 * p.tiles * (p.many ? kManyWaves : 1);
     const int span = p.many ? span_of(p.pad_dim) : kStep;
     // workgroups that fit the chip at once, fewer where the steps are fewer
     const int64_t tiles = (n * group + r - 1) / r + seqs;
     const int64_t steps = (max_tokens + span - 1) / span;
     const int64_t units = p.units = tiles * kv_heads * (steps > 0 ? steps : 1);
-    const int64_t fit = 256 * waves_of(p.pad_dim, p.tiles, p.many);
+    const int64_t fit = 256 * waves_of(p.pad_dim, p.tiles, p.many) * 4 / (p.many ? kManyWaves : kWaves);
     p.blocks = (int)(units < fit ? (units + 7) / 8 * 8 : fit);
     if (p.blocks < 8) p.blocks = 8;
     p.workspace_floats = (int64_t)p.blocks * ((int64_t)sizeof(Desc) / 4 + 2 * r * 2 + 2 * r * p.pad_dim);
