@@ -46,7 +46,6 @@ typedef uint32_t u32x4_kv __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kManyWaves = 8;               // of the many-rows kernel
 constexpr int kTile = 32;                   // tokens of a wave's step
 constexpr int kStep = kTile * kWaves;       // tokens of a workgroup's step
 constexpr float kNone = -1e30f;             // M of a row that has seen nothing
@@ -58,13 +57,7 @@ constexpr int span_of(int pad_dim) { return pad_dim == 256 ? 32 : 64; }
 // Waves a SIMD that the registers leave room for.
 constexpr int waves_of(int pad_dim, int tiles, bool many)
 {
-    return many ? (pad_dim == 256 || tiles == 2 ? 2 : 4) : pad_dim == 256 ? 1 : tiles == 2 ? 2 : 3;
-}
-
-// The most 16-row tiles a wave holds without spilling.
-constexpr int tiles_of(int pad_dim, int dtype, bool many)
-{
-    return pad_dim == 256 ? 1 : 2;
+    return many ? 2 : pad_dim == 256 ? 1 : tiles == 2 ? 2 : 3;
 }
 
 // Tables that no kernel of the call writes, read through the scalar cache
@@ -128,6 +121,14 @@ __device__ __forceinline__ Work work_of(const KvAttentionArgs& a, const Seq& s, 
 template <int BITS>
 constexpr float kOffset = BITS == 4 ? 24.f : 640.f;
 
+// -offset twice in fp16
+template <int BITS>
+constexpr uint32_t kBack = BITS == 4 ? 0xce00ce00u : 0xe100e100u;
+
+__device__ __forceinline__ float key_scale(uint32_t u) { return __uint_as_float(u << 16); }
+// a zero vector's scale as 2^-70 (its points are zeros): no infinity times zero in the weights
+__device__ __forceinline__ float value_scale(uint32_t u) { return __uint_as_float(max(u & 0xffff0000u, 0x1c800000u)); }
+
 __device__ __forceinline__ uint32_t minus(uint32_t u, float off)
 {
     const half2_kv o = {(_Float16)off, (_Float16)off};
@@ -171,15 +172,16 @@ __device__ __forceinline__ void key_operand(const uint32_t* w, uint32_t (&r)[4])
 
 // Coordinates of one block of two tokens as centred fp16 pairs: register e
 // holds coordinate e (E = 8), or e + 4 * upper (E = 4).
-template <int BITS, int E>
+template <int BITS, int E, bool CENTER>
 __device__ __forceinline__ void value_pair(const uint32_t* a, const uint32_t* b, bool upper, uint32_t (&r)[E])
 {
     if constexpr (BITS == 4) {
         const uint32_t lo = __builtin_amdgcn_perm(b[0], a[0], 0x05040100u);
         const uint32_t hi = __builtin_amdgcn_perm(b[0], a[0], 0x07060302u);
-        uint32_t z = lo ^ hi;   // lowest bits of the fields, at 0, 4, 8, 12 of each half
-        z ^= z << 8;
-        z ^= z << 4;
+        // lowest bits of the fields, at 0, 4, 8, 12 of each half; their sum's parity arrives at 12
+        uint32_t z = (lo ^ hi) & 0x11111111u;
+        z += z << 8;
+        z += z << 4;
         const uint32_t base = 0x4c004c00u | ((hi >> 7) & 0x00200020u);
         const uint32_t fixed = hi ^ (z & 0x10001000u);
         if constexpr (E == 8) {
@@ -214,8 +216,9 @@ __device__ __forceinline__ void value_pair(const uint32_t* a, const uint32_t* b,
             r[7] = (__builtin_amdgcn_perm(hb, ha, 0x0c070c03u) << 1) | base;
         }
     }
+    if constexpr (CENTER)
 #pragma unroll
-    for (int e = 0; e < E; ++e) r[e] = minus(r[e], kOffset<BITS>);
+        for (int e = 0; e < E; ++e) r[e] = minus(r[e], kOffset<BITS>);
 }
 
 // What a wave loads for 16 tokens: a lane's blocks of one key, four tokens'
@@ -324,55 +327,110 @@ template <int DP, int BITS, int NR, int DT, bool QS, bool PS>
 struct Rows {
     static constexpr int C = DP / 32, NT = DP / 16;
     uint32_t q_hi[NR][C][4], q_lo[NR][QS ? C : 1][4];
-    float scale[NR], bias[NR];   // of the scores; what the keys' offset adds to them, negated
-    int limit[NR], own[NR];      // a row sees tokens below limit; own: its query token, -1 for none
+    float bias[NR];              // what the keys' offset adds to the scores, negated
+    int limit[NR], own[NR];      // a row sees tokens below limit; own: its query token
     uint64_t drafts[NR];         // its row of the mask, the first word
     float M[NR], l[NR];
     f32x4_kv o[NR][NT];
 
-    // first: the wave's first row in the segment's (token, head of the group)
-    // rows; meanwhile: what may be loaded while the rows are on their way
-    template <class F>
-    __device__ __forceinline__ void begin(const KvAttentionArgs& a, const Seq& sq, int kh, int first, int lane, F meanwhile)
+    // The rows as they lie in memory.  first: the wave's first row in the
+    // segment's (token, head of the group) rows.  Rows past the last one read
+    // that one again and see nothing.
+    static constexpr int kRaw = DT == DT_F32 ? 2 : 1;
+    struct Raw {
+        u32x4_kv x[NR][C][kRaw];
+    };
+    __device__ __forceinline__ void load(const KvAttentionArgs& a, const Seq& sq, int kh, int first, int lane, Raw& raw)
     {
         const int g = lane >> 4, n = lane & 15;
         const int ctx = sq.length - sq.tokens, rows = sq.tokens * a.group;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            const int row = first + 16 * r + n;
-            const bool on = row < rows;
+            const bool on = first + 16 * r + n < rows;
+            const int row = min(first + 16 * r + n, rows - 1);
             const uint32_t t = u32div((uint32_t)row, a.group_div);
             const int hq = kh * a.group + (row - (int)t * a.group);
-            own[r] = on ? sq.token0 + (int)t : -1;
-            limit[r] = on ? (a.mask ? ctx : min(sq.length, ctx + (int)t + 1)) : 0;
-            drafts[r] = a.mask && on ? (uint64_t)a.mask[(int64_t)own[r] * a.mask_words] : 0;
-            float x[C][8];
+            own[r] = sq.token0 + (int)t;
+            limit[r] = on ? (a.mask ? ctx : min(sq.length, ctx + (int)t + 1)) : -0x40000000;
+            const int64_t at = (int64_t)own[r] * a.q_tok + hq * a.q_head;
+            drafts[r] = 0;
+            if (a.mask && on) drafts[r] = (uint64_t)a.mask[(int64_t)own[r] * a.mask_words];
+            if (a.vec) {
+                const char* p = reinterpret_cast<const char*>(a.q) + at * (kRaw * 2);
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int block = C * g + c;
+                for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[c][j] = 0.f;
-                if (on && block < (a.c.dim >> 3))
-                    load_n<DT, 8>(a.q, (int64_t)own[r] * a.q_tok + hq * a.q_head + 8 * block, a.vec, x[c]);
+                    for (int i = 0; i < kRaw; ++i)
+                        raw.x[r][c][i] = *reinterpret_cast<const u32x4_kv*>(p + 16 * kRaw * min(C * g + c, (a.c.dim >> 3) - 1) + 16 * i);
+            } else {
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const int64_t e = at + 8 * min(C * g + c, (a.c.dim >> 3) - 1);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if constexpr (DT == DT_F32) {
+                            raw.x[r][c][0][j] = reinterpret_cast<const uint32_t*>(a.q)[e + j];
+                            raw.x[r][c][1][j] = reinterpret_cast<const uint32_t*>(a.q)[e + 4 + j];
+                        } else {
+                            const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + e + 2 * j;
+                            raw.x[r][c][0][j] = (uint32_t)p[0] | (uint32_t)p[1] << 16;
+                        }
+                    }
+                }
             }
-            if (r == NR - 1) meanwhile();
-            float top = 0.f;
+        }
+    }
+
+    // element j of a row's block c in fp32; zero past dim
+    __device__ __forceinline__ static float value(const KvAttentionArgs& a, const Raw& raw, int r, int c, int j, int g)
+    {
+        float x, y;
+        if constexpr (DT == DT_F32) {
+            x = __uint_as_float(raw.x[r][c][j >> 2][j & 3]);
+        } else {
+            unpack2<DT>(raw.x[r][c][0][j >> 1], x, y);
+            if (j & 1) x = y;
+        }
+        return C * g + c < (a.c.dim >> 3) ? x : 0.f;
+    }
+
+    // The largest finite row maximum, as bits, over the wave.
+    __device__ __forceinline__ static uint32_t top(const KvAttentionArgs& a, const Raw& raw, int g)
+    {
+        uint32_t most = 0;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            uint32_t t = 0;
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[c][j]));
-            top = over_groups_max(top);
-            // times 2^k, which brings the row's largest value to [2^10, 2^11)
-            const int e = max((int)(__float_as_uint(top) >> 23), 20);
-            const float up = copysignf(__uint_as_float((uint32_t)(264 - e) << 23), a.scale);
-            // above zero, so that a hidden token's score stays at minus infinity
-            scale[r] = fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(e - 10) << 23), 0x1p-126f);
+                for (int j = 0; j < 8; ++j) t = max(t, __float_as_uint(value(a, raw, r, c, j, g)) & 0x7fffffffu);
+            t = max(t, (uint32_t)__shfl_xor((int)t, 16, 64));
+            t = max(t, (uint32_t)__shfl_xor((int)t, 32, 64));
+            most = max(most, t < 0x7f800000u ? t : 0u);
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
+        return most;
+    }
+
+    // To fp16 times 2^k, which brings the workgroup's largest value (bits
+    // `most`) to [2^13, 2^14): one factor for all rows, so that it joins the
+    // keys' scales.  What a small row loses is 2^-38 of the largest one in
+    // absolute terms, far below the rounding of that one's scores.  Returns
+    // what the scores are multiplied by.
+    __device__ __forceinline__ float convert(const KvAttentionArgs& a, const Raw& raw, uint32_t most, int g)
+    {
+        const int e = max((int)(most >> 23), 24);
+        const float up = copysignf(__uint_as_float((uint32_t)(267 - e) << 23), a.scale);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
             float sum = 0.f;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float u = x[c][i] * up, v = x[c][i + 4] * up;
+                    const float u = value(a, raw, r, c, i, g) * up, v = value(a, raw, r, c, i + 4, g) * up;
                     q_hi[r][c][i] = pack2<DT_F16>(u, v);
                     float hu, hv;
                     unpack2<DT_F16>(q_hi[r][c][i], hu, hv);
@@ -386,6 +444,8 @@ struct Rows {
 #pragma unroll
             for (int j = 0; j < NT; ++j) o[r][j] = f32x4_kv{0.f, 0.f, 0.f, 0.f};
         }
+        // above zero, so that a hidden token's score stays at minus infinity
+        return fmaxf(fabsf(a.scale) * __uint_as_float((uint32_t)(e - 13) << 23), 0x1p-126f);
     }
 
     // s += the keys' chunk c times the rows
@@ -404,62 +464,61 @@ struct Rows {
         }
     }
 
-    // The weights of 32 tokens from their scores s and scale words sc, as the
-    // second product's B operand.  whole: every row sees all of them.
+    // The weights of 32 tokens as the second product's B operand, from their
+    // scores s, the keys' scales times the scores' factor and the values'
+    // scales.  whole: every row sees all of them.
     __device__ __forceinline__ void weigh(const KvAttentionArgs& a, const Seq& sq, const f32x4_kv (&s)[2][NR],
-                                          const uint32_t (&sc)[2][4], int token, bool whole, int g,
+                                          const float (&bk)[8], const float (&bv)[8], int token, bool whole, int g,
                                           uint32_t (&p_hi)[NR][4], uint32_t (&p_lo)[NR][4])
     {
-        float bk[8], bv[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t u = sc[i >> 2][i & 3];
-            bk[i] = __uint_as_float(u << 16);
-            // a zero vector's scale as 2^-70 (its points are zeros): no infinity times zero below
-            bv[i] = __uint_as_float(max(u & 0xffff0000u, 0x1c800000u));
-        }
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            float u[8], w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] = s[i >> 2][r][i & 3] * bk[i];
             uint32_t seen = 0xffu;
-            if (!whole) {
+            if (!whole)
                 seen = seen_of(a, sq, limit[r], own[r], drafts[r], token + 4 * g) |
                        seen_of(a, sq, limit[r], own[r], drafts[r], token + 16 + 4 * g) << 4;
+            float w[8], sum;
+            // a second time where the reference M had to move (and no third,
+            // whatever the scores)
+            // the weights with respect to M; returns the lane's largest
+            auto attempt = [&]() {
+                float t[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) u[i] = seen >> i & 1u ? u[i] : -INFINITY;
-            }
-            float sum = 0.f, top = 0.f;
+                for (int i = 0; i < 8; ++i) t[i] = fmaf(s[i >> 2][r][i & 3], bk[i], -M[r]);
+                if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(u[i], scale[r], -M[r]));
-                sum += p;
-                w[i] = p * bv[i];
-            }
-            if (!whole) {   // zero times a NaN scale
+                    for (int i = 0; i < 8; ++i) t[i] = seen >> i & 1u ? t[i] : -INFINITY;
+                }
+                float top = 0.f;
+                sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = seen >> i & 1u ? w[i] : 0.f;
-            }
+                for (int i = 0; i < 8; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(t[i]);
+                    sum += p;
+                    w[i] = p * bv[i];
+                }
+                if (!whole) {   // zero times the scale of a hidden token, which may be NaN
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, w[i]);
-            if (__any(top > kDue)) {
+                    for (int i = 0; i < 8; ++i) w[i] = seen >> i & 1u ? w[i] : 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, w[i]);
+                return top;
+            };
+            if (__any(attempt() > kDue)) {
                 float most = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) most = fmaxf(most, fmaf(u[i], scale[r], __builtin_amdgcn_logf(bv[i])));
+                for (int i = 0; i < 8; ++i) {
+                    const float at = fmaf(s[i >> 2][r][i & 3], bk[i], __builtin_amdgcn_logf(bv[i]));
+                    most = fmaxf(most, seen >> i & 1u ? at : -INFINITY);
+                }
                 const float to = fmaxf(M[r], over_groups_max(most) - kSettle);
                 const float f = __builtin_amdgcn_exp2f(M[r] - to);
                 M[r] = to;
                 l[r] *= f;
 #pragma unroll
                 for (int j = 0; j < NT; ++j) o[r][j] *= f;
-                sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(u[i], scale[r], -to));
-                    sum += p;
-                    w[i] = seen >> i & 1u ? p * bv[i] : 0.f;
-                }
+                attempt();
             }
             l[r] += sum;
 #pragma unroll
@@ -613,6 +672,15 @@ struct Pages {
     }
 };
 
+// The same value, but not one that the compiler can compute ahead of the
+// loops: what a segment's beginning and end derive from the lane would else be
+// kept in registers through the steps.
+__device__ __forceinline__ int here(int v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 __device__ __forceinline__ int xcd_id()
 {
     // neighbouring runs on one XCD (workgroups go to the 8 XCDs in turn)
@@ -632,6 +700,12 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
     constexpr int E = DP == 64 ? 4 : 8;          // a lane's coordinates of a value block
     constexpr int kRows = 16 * NR;
     constexpr int kPitch = DP + 4;
+    // The values' offset leaves in a second product of the same step (four
+    // times fewer cycles on the matrix cores, which are idle, than as packed
+    // subtractions), so the sum is off by 2^-24 of one step's offset, 2^-19 of
+    // the values' largest; only bf16 results may be off by as much, the others
+    // subtract it from the operand, which is exact.
+    constexpr bool kCenter = DT != DT_BF16;
     __shared__ __align__(16) float sh_o[kWaves][16 * kPitch];
     __shared__ float sh_m[kWaves][kRows], sh_l[kWaves][kRows];
 
@@ -665,8 +739,9 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
         uint32_t kw[2][C * W], vw[2][T::B][4 * W], sc[2][4];
         int64_t at[2];
         R rs;
-        rs.begin(a, sq, kh, row0, lane, [&]() {
-            if (token >= stop) return;
+        typename R::Raw raw;
+        rs.load(a, sq, kh, row0, here(lane), raw);
+        if (token < stop) {
             at[0] = pages.row(a, token);
             at[1] = pages.row(a, token + 16 < reach ? token + 16 : token);
 #pragma unroll
@@ -675,7 +750,8 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
             for (int h = 0; h < 2; ++h) words.scales(a.c, at[h], sc[h]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.values(a.c, at[h], vw[h]);
-        });
+        }
+        const float factor = rs.convert(a, raw, R::top(a, raw, g), g);
         for (; token < stop; token += kStep) {
             const int ahead = token + kStep < stop ? token + kStep : token;
             at[0] = pages.row(a, ahead);
@@ -694,24 +770,34 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.keys(a.c, at[h], kw[h]);
-            uint32_t p_hi[NR][4], p_lo[NR][4];
-            rs.weigh(a, sq, s, sc, token, token + kTile <= all, g, p_hi, p_lo);
+            float bk[8], bv[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                bk[i] = key_scale(sc[i >> 2][i & 3]) * factor;
+                bv[i] = value_scale(sc[i >> 2][i & 3]);
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.scales(a.c, at[h], sc[h]);
+            uint32_t p_hi[NR][4], p_lo[NR][4];
+            rs.weigh(a, sq, s, bk, bv, token, token + kTile <= all, g, p_hi, p_lo);
 #pragma unroll
             for (int blk = 0; blk < T::B; ++blk) {
                 uint32_t v[4][E];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    value_pair<BITS, E>(&vw[i >> 1][blk][(i & 1) * 2 * W], &vw[i >> 1][blk][((i & 1) * 2 + 1) * W], n >= 8, v[i]);
+                    value_pair<BITS, E, kCenter>(&vw[i >> 1][blk][(i & 1) * 2 * W], &vw[i >> 1][blk][((i & 1) * 2 + 1) * W], n >= 8, v[i]);
 #pragma unroll
-                for (int e = 0; e < E; ++e) rs.add(u32x4_kv{v[0][e], v[1][e], v[2][e], v[3][e]}, blk * 8 + e, p_hi, p_lo);
+                for (int e = 0; e < E; ++e) {
+                    rs.add(u32x4_kv{v[0][e], v[1][e], v[2][e], v[3][e]}, blk * 8 + e, p_hi, p_lo);
+                    if constexpr (!kCenter) rs.add(u32x4_kv{kBack<BITS>, kBack<BITS>, kBack<BITS>, kBack<BITS>}, blk * 8 + e, p_hi, p_lo);
+                }
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.values(a.c, at[h], vw[h]);
         }
 
         // the four waves' rows
+        const int tid = here(threadIdx.x), g = (tid & 63) >> 4, n = tid & 15;
         const bool done = count == ln.wk.steps;
         const int64_t slot = 2 * id + (ln.step == 0 ? 1 : 0);
 #pragma unroll
@@ -736,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
                     *reinterpret_cast<f32x4_kv*>(&sh_o[wave][n * kPitch + R::place(i, q, g)]) = rs.piece(r, i, q) * f;
             __syncthreads();
             // 16 rows x DP: a thread takes DP / 16 neighbours of one row in pieces of 8
-            const int row = threadIdx.x >> 4;
+            const int row = tid >> 4;
             const int rr = 16 * r + row;
             float mm = sh_m[0][rr];
 #pragma unroll
@@ -749,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
                 const int hq = kh * a.group + (row0 + rr - (int)t * a.group);
                 const int64_t at = ((int64_t)sq.token0 + t) * a.heads + hq;
                 const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
-                for (int d = 8 * (threadIdx.x & 15); d < a.c.dim; d += 128) {
+                for (int d = 8 * (tid & 15); d < a.c.dim; d += 128) {
                     float x[8];
 #pragma unroll
                     for (int j = 0; j < 8; j += 4) {
@@ -768,7 +854,7 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
                         store_n<DT_F32, 8>(parts.o, (slot * kRows + rr) * DP + d, x);
                     }
                 }
-                if ((threadIdx.x & 15) == 0) {
+                if ((tid & 15) == 0) {
                     if (done) {
                         if (a.lse) a.lse[at] = ll > 0.f || ll != ll ? (mm + log2f(ll)) * (1.f / kLog2e) : -INFINITY;
                     } else {
@@ -783,22 +869,28 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
     } while (ln.next(a, count, kRows, kStep));
 }
 
-// More rows: eight waves hold 16 * NR rows each and share the tokens, which
-// they decode once into operands in LDS, an eighth each: one buffer is filled
-// while the other one is used.
-template <int DP, int BITS, int NR, int DT, bool QS, bool PS, int OCC>
-__global__ void __launch_bounds__(64 * kManyWaves, OCC) kv_many_kernel(KvAttentionArgs a, int most_parts)
+// More rows: WAVES waves hold 16 * NR rows each and share the tokens, which
+// they decode once into operands in LDS, an equal part each: one buffer is
+// filled while the other one is used.
+template <int DP, int BITS, int NR, int WAVES, int DT, bool QS, bool PS, int OCC>
+__global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArgs a, int most_parts)
 {
     using R = Rows<DP, BITS, NR, DT, QS, PS>;
     constexpr int C = R::C, NT = R::NT, W = BITS / 4;
-    constexpr int kRows = 16 * NR * kManyWaves;
+    constexpr int kRows = 16 * NR * WAVES;
     constexpr int kSpan = span_of(DP);              // tokens of a step
     constexpr int kSub = kSpan / 16;
-    constexpr int kPieces = kManyWaves / kSub;      // waves that share 16 tokens' keys and values
-    static_assert(DP == 64 ? kPieces == 2 : C == 2 * kPieces, "two key chunks a wave");
+    constexpr int kPieces = WAVES / kSub;           // waves that share 16 tokens' keys and values
+    // A wave's piece of 16 tokens: KC chunks of the keys and VE of a lane's
+    // coordinates of the values (DP = 64 in two pieces: the keys, the values).
+    constexpr bool kApart = DP == 64 && kPieces == 2;
+    constexpr int KC = kApart ? C : C / kPieces;
+    constexpr int VE = kApart || DP == 64 ? 4 : DP / 16 / kPieces;
+    static_assert(kPieces >= 1 && (VE == 4 || VE == 8), "");
     __shared__ __align__(16) u32x4_kv sh_k[2][kSub][C][64];
     __shared__ __align__(16) u32x4_kv sh_v[2][kSub / 2][NT][64];
-    __shared__ __align__(16) uint32_t sh_s[2][kSpan];
+    __shared__ __align__(16) float sh_bk[2][kSpan], sh_bv[2][kSpan];   // keys' scales times the scores' factor, values'
+    __shared__ uint32_t sh_top[WAVES];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
@@ -810,17 +902,14 @@ __global__ void __launch_bounds__(64 * kManyWaves, OCC) kv_many_kernel(KvAttenti
     if (most_parts > 1 && threadIdx.x == 0) parts.descs[id].parts = 0;
     if (!some) return;
 
-    // A wave's piece of 16 tokens: two chunks of the keys (DP = 64: piece 0
-    // takes both, piece 1 the values) and four coordinates of a block of the
-    // values, upper or lower.
-    const bool has_keys = DP > 64 || piece == 0, has_values = DP > 64 || piece == 1;
+    const bool has_keys = !kApart || piece == 0, has_values = !kApart || piece == 1;
     const int nb = a.c.dim >> 3, row_bytes = 4 * nb * W;
-    const int chunk = DP > 64 ? 2 * piece : 0;
-    const uint32_t k_at = n * row_bytes + 4 * W * min(C * g + chunk, nb - 2);
-    const int blk = DP == 256 ? piece >> 1 : 0;
+    const int chunk = kApart ? 0 : KC * piece;
+    const uint32_t k_at = n * row_bytes + 4 * W * min(C * g + chunk, nb - KC);
+    const int blk = DP == 256 ? VE * piece / 8 : 0;
     const uint32_t v_at = 4 * g * row_bytes + 16 * W * min(DP == 64 ? n & 7 : 16 * blk + n, nb - 1);
-    const bool upper = DP == 64 ? n >= 8 : piece & 1;
-    const int v_tile = DP == 64 ? 0 : 8 * blk + 4 * (piece & 1);
+    const bool upper = DP == 64 ? n >= 8 : piece & 1;   // where VE = 4
+    const int v_tile = kApart ? 0 : VE * piece;
 
     int count;
     do {
@@ -838,20 +927,23 @@ __global__ void __launch_bounds__(64 * kManyWaves, OCC) kv_many_kernel(KvAttenti
         int token = ln.step * kSpan;
         const int stop = min((ln.step + count) * kSpan, reach);
 
-        uint32_t kw[2 * W], vw[4 * W], sw;
-        auto fetch = [&](int from) {
-            const int t = from + 16 * sub;
-            const int64_t row = pages.row(a, t < reach ? t : from);
+        uint32_t kw[KC * W], vw[4 * W], sw;
+        float factor = 0.f;
+        auto row_of = [&](int from) { return pages.row(a, from + 16 * sub < reach ? from + 16 * sub : from); };
+        auto fetch = [&](int64_t row) {
             if (has_keys) {
                 const char* p = reinterpret_cast<const char*>(a.c.k) + row * row_bytes + k_at;
-                if constexpr (W == 1) {
+                if constexpr (KC * W == 2) {
                     const uint2 u = *reinterpret_cast<const uint2*>(p);
                     kw[0] = u.x;
                     kw[1] = u.y;
                 } else {
-                    const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(p);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) kw[j] = u[j];
+                    for (int i = 0; i < KC * W / 4; ++i) {
+                        const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(p + 16 * i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) kw[4 * i + j] = u[j];
+                    }
                 }
             }
             if (has_values) {
@@ -868,32 +960,45 @@ __global__ void __launch_bounds__(64 * kManyWaves, OCC) kv_many_kernel(KvAttenti
         auto decode = [&](int buf) {
             if (has_keys) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int c = 0; c < KC; ++c) {
                     uint32_t k[4];
                     key_operand<BITS, QS>(&kw[c * W], k);
                     sh_k[buf][sub][chunk + c][lane] = u32x4_kv{k[0], k[1], k[2], k[3]};
                 }
             }
             if (has_values) {
-                uint32_t v[2][4];
-                value_pair<BITS, 4>(&vw[0], &vw[W], upper, v[0]);
-                value_pair<BITS, 4>(&vw[2 * W], &vw[3 * W], upper, v[1]);
+                uint32_t v[2][VE];
+                value_pair<BITS, VE, true>(&vw[0], &vw[W], upper, v[0]);
+                value_pair<BITS, VE, true>(&vw[2 * W], &vw[3 * W], upper, v[1]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                for (int e = 0; e < VE; ++e)
                     reinterpret_cast<uint2*>(&sh_v[buf][sub >> 1][v_tile + e][lane])[sub & 1] = make_uint2(v[0][e], v[1][e]);
             }
-            if (piece == 0 && lane < 16) sh_s[buf][16 * sub + lane] = sw;
+            if (piece == 0 && lane < 16) {
+                sh_bk[buf][16 * sub + lane] = key_scale(sw) * factor;
+                sh_bv[buf][16 * sub + lane] = value_scale(sw);
+            }
         };
         R rs;
-        rs.begin(a, sq, kh, first, lane, [&]() {
-            if (token < stop) fetch(token);
-        });
+        typename R::Raw raw;
+        rs.load(a, sq, kh, first, here(lane), raw);
+        if (token < stop) fetch(row_of(token));
+        {
+            const uint32_t t = R::top(a, raw, g);
+            if (lane == 0) sh_top[wave] = t;
+            __syncthreads();
+            uint32_t most = sh_top[0];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) most = max(most, sh_top[w]);
+            factor = rs.convert(a, raw, most, g);
+        }
         if (token < stop) {
             decode(0);
-            if (token + kSpan < stop) fetch(token + kSpan);
+            if (token + kSpan < stop) fetch(row_of(token + kSpan));
         }
         __syncthreads();
         for (int buf = 0; token < stop; token += kSpan, buf ^= 1) {
+            const int64_t beyond = row_of(min(token + 2 * kSpan, stop - 1) & ~15);
 #pragma unroll
             for (int p = 0; p < kSub / 2; ++p) {
                 const int at = token + kTile * p;
@@ -906,26 +1011,31 @@ __global__ void __launch_bounds__(64 * kManyWaves, OCC) kv_many_kernel(KvAttenti
 #pragma unroll
                     for (int c = 0; c < C; ++c) rs.score(s[h], sh_k[buf][2 * p + h][c][lane], c);
                 }
-                uint32_t sc[2][4];
+                float bk[8], bv[8];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const u32x4_kv u = *reinterpret_cast<const u32x4_kv*>(&sh_s[buf][16 * (2 * p + h) + 4 * g]);
+                    const f32x4_kv x = *reinterpret_cast<const f32x4_kv*>(&sh_bk[buf][16 * (2 * p + h) + 4 * g]);
+                    const f32x4_kv y = *reinterpret_cast<const f32x4_kv*>(&sh_bv[buf][16 * (2 * p + h) + 4 * g]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) sc[h][j] = u[j];
+                    for (int j = 0; j < 4; ++j) {
+                        bk[4 * h + j] = x[j];
+                        bv[4 * h + j] = y[j];
+                    }
                 }
                 uint32_t p_hi[NR][4], p_lo[NR][4];
-                rs.weigh(a, sq, s, sc, at, at + kTile <= all, g, p_hi, p_lo);
+                rs.weigh(a, sq, s, bk, bv, at, at + kTile <= all, g, p_hi, p_lo);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) rs.add(sh_v[buf][p][j][lane], j, p_hi, p_lo);
             }
             if (token + kSpan < stop) {
                 decode(buf ^ 1);
-                if (token + 2 * kSpan < stop) fetch(token + 2 * kSpan);
+                if (token + 2 * kSpan < stop) fetch(beyond);
             }
             __syncthreads();
         }
 
         const bool done = count == ln.wk.steps;
+        const int tid = here(threadIdx.x), g = (tid & 63) >> 4, n = tid & 15;
         const int64_t slot = 2 * id + (ln.step == 0 ? 1 : 0);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
@@ -1013,17 +1123,18 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(KvAttentionArgs a, in
     if (a.lse && across == 0) a.lse[at] = some ? (m + log2f(l)) * (1.f / kLog2e) : -INFINITY;
 }
 
-template <int DP, int BITS, int NR, int DT, bool MANY>
+template <int DP, int BITS, int NR, int WAVES, int DT>
 hipError_t launch(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_t s)
 {
     constexpr bool QS = DT == DT_F32, PS = DT != DT_BF16;
-    constexpr int OCC = waves_of(DP, NR, MANY);
-    constexpr int kRows = 16 * NR * (MANY ? kManyWaves : 1);
+    constexpr bool kMany = WAVES > 0;
+    constexpr int OCC = waves_of(DP, NR, kMany);
+    constexpr int kRows = 16 * NR * (kMany ? WAVES : 1);
     const int64_t most_tokens = (int64_t)a.max_pages * a.c.page_size;
-    const int span = MANY ? span_of(DP) : kStep;
+    const int span = kMany ? span_of(DP) : kStep;
     const int most_parts = (int)((most_tokens + span - 1) / span);
-    if constexpr (MANY)
-        hipLaunchKernelGGL((kv_many_kernel<DP, BITS, NR, DT, QS, PS, OCC>), dim3(p.blocks), dim3(64 * kManyWaves), 0, s, a, most_parts);
+    if constexpr (kMany)
+        hipLaunchKernelGGL((kv_many_kernel<DP, BITS, NR, WAVES, DT, QS, PS, OCC>), dim3(p.blocks), dim3(64 * WAVES), 0, s, a, most_parts);
     else
         hipLaunchKernelGGL((kv_few_kernel<DP, BITS, NR, DT, QS, PS, OCC>), dim3(p.blocks), dim3(kThreads), 0, s, a, most_parts);
     hipError_t e = hipGetLastError();
@@ -1038,16 +1149,16 @@ hipError_t launch(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_
 template <int DP, int BITS, int DT>
 hipError_t by_tiles(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_t s)
 {
-    if (!p.many) {
-        if (p.tiles == 1) return launch<DP, BITS, 1, DT, false>(a, p, s);
-        if constexpr (tiles_of(DP, DT, false) >= 2) {
-            if (p.tiles == 2) return launch<DP, BITS, 2, DT, false>(a, p, s);
-        }
+    if constexpr (DP == 256) {
+        if (p.waves == 0 && p.tiles == 1) return launch<DP, BITS, 1, 0, DT>(a, p, s);
+        if (p.waves == 4 && p.tiles == 1) return launch<DP, BITS, 1, 4, DT>(a, p, s);
+        if (p.waves == 8 && p.tiles == 1) return launch<DP, BITS, 1, 8, DT>(a, p, s);
     } else {
-        if (p.tiles == 1) return launch<DP, BITS, 1, DT, true>(a, p, s);
-        if constexpr (tiles_of(DP, DT, true) >= 2) {
-            if (p.tiles == 2) return launch<DP, BITS, 2, DT, true>(a, p, s);
-        }
+        if (p.waves == 0 && p.tiles == 1) return launch<DP, BITS, 1, 0, DT>(a, p, s);
+        if (p.waves == 0 && p.tiles == 2) return launch<DP, BITS, 2, 0, DT>(a, p, s);
+        if (p.waves == 4 && p.tiles == 1) return launch<DP, BITS, 1, 4, DT>(a, p, s);
+        if (p.waves == 4 && p.tiles == 2) return launch<DP, BITS, 2, 4, DT>(a, p, s);
+        if (p.waves == 8 && p.tiles == 2) return launch<DP, BITS, 2, 8, DT>(a, p, s);
     }
     return hipErrorInvalidValue;
 }
@@ -1073,17 +1184,24 @@ KvAttentionPlan kv_attention_plan(int64_t n, int seqs, int heads, int kv_heads, 
     p.pad_dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
     const int64_t group = heads / kv_heads;
     const int64_t rows = (n + seqs - 1) / seqs * group;   // of a sequence, on average
-    p.many = rows > 32;
-    p.tiles = p.many ? (rows > 128 ? 2 : 1) : (rows > 16 ? 2 : 1);
-    const int most = tiles_of(p.pad_dim, dtype, p.many);
-    if (p.tiles > most) p.tiles = most;
-    const int64_t r = 16 * p.tiles * (p.many ? kManyWaves : 1);
-    const int span = p.many ? span_of(p.pad_dim) : kStep;
+    if (rows <= 16 || (rows <= 32 && p.pad_dim < 256)) {
+        p.waves = 0;
+        p.tiles = rows <= 16 ? 1 : 2;
+    } else if (p.pad_dim == 256) {
+        p.waves = rows <= 64 ? 4 : 8;
+        p.tiles = 1;
+    } else {
+        p.waves = rows <= 128 ? 4 : 8;
+        p.tiles = rows <= 64 ? 1 : 2;
+    }
+    const bool many = p.waves > 0;
+    const int64_t r = 16 * p.tiles * (many ? p.waves : 1);
+    const int span = many ? span_of(p.pad_dim) : kStep;
     // workgroups that fit the chip at once, fewer where the steps are fewer
     const int64_t tiles = (n * group + r - 1) / r + seqs;
     const int64_t steps = (max_tokens + span - 1) / span;
     const int64_t units = p.units = tiles * kv_heads * (steps > 0 ? steps : 1);
-    const int64_t fit = 256 * waves_of(p.pad_dim, p.tiles, p.many) * 4 / (p.many ? kManyWaves : kWaves);
+    const int64_t fit = 256 * waves_of(p.pad_dim, p.tiles, many) * 4 / (many ? p.waves : kWaves);
     p.blocks = (int)(units < fit ? (units + 7) / 8 * 8 : fit);
     if (p.blocks < 8) p.blocks = 8;
     p.workspace_floats = (int64_t)p.blocks * ((int64_t)sizeof(Desc) / 4 + 2 * r * 2 + 2 * r * p.pad_dim);

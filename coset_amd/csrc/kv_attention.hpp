@@ -35,7 +35,7 @@ struct KvAttentionArgs {
 
 // How a call is cut.
 struct KvAttentionPlan {
-    bool many;      // the kernel whose waves share the tokens (else each has its own)
+    int waves;      // of a workgroup of the kernel whose waves share the tokens: 4 or 8; 0: each has its own
     int tiles;      // 16-row tiles of query rows (token x head of a group) that a wave holds: 1 or 2
     int blocks;
     int pad_dim;    // 64, 128 or 256
