@@ -126,13 +126,30 @@ template <int BITS>
 constexpr uint32_t kBack = BITS == 4 ? 0xce00ce00u : 0xe100e100u;
 
 __device__ __forceinline__ float key_scale(uint32_t u) { return __uint_as_float(u << 16); }
-// a zero vector's scale as 2^-70 (its points are zeros): no infinity times zero in the weights
-__device__ __forceinline__ float value_scale(uint32_t u) { return __uint_as_float(max(u & 0xffff0000u, 0x1c800000u)); }
+__device__ __forceinline__ float value_scale(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
 __device__ __forceinline__ uint32_t minus(uint32_t u, float off)
 {
     const half2_kv o = {(_Float16)off, (_Float16)off};
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_kv, u) - o);
+}
+
+// All ones where bit BIT of u is set (one instruction; the compiler would
+// compare and select).
+template <int BIT>
+__device__ __forceinline__ uint32_t spread(uint32_t u)
+{
+    uint32_t r;
+    asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(r) : "v"(u), "n"(BIT));
+    return r;
+}
+
+// a ^ (b & c)
+__device__ __forceinline__ uint32_t flip(uint32_t a, uint32_t b, uint32_t c)
+{
+    uint32_t r;
+    asm("v_bitop3_b32 %0, %1, %2, %3 bitop3:0x78" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
 }
 
 // Nibble fields sit at bits 6..9 of a half whose exponent is that of [16, 32):
@@ -149,16 +166,15 @@ template <int BITS, bool CENTER>
 __device__ __forceinline__ void key_operand(const uint32_t* w, uint32_t (&r)[4])
 {
     if constexpr (BITS == 4) {
-        const uint32_t base = ((uint32_t)__builtin_amdgcn_sbfe((int)w[0], 28, 1) & 0x00200020u) | 0x4c004c00u;
+        const uint32_t base = (spread<28>(w[0]) & 0x00200020u) | 0x4c004c00u;
         r[0] = nibbles<0>(w[0], base);
         r[1] = nibbles<1>(w[0], base);
         r[2] = nibbles<2>(w[0], base);
         // n_7's lowest bit, at 22 here: h there, xor the parity of the word's lowest bits
-        r[3] = nibbles<3>(w[0], base) ^ ((uint32_t)__popc(w[0] & 0x11111111u) << 22 & 0x00400000u);
+        r[3] = flip(nibbles<3>(w[0], base), (uint32_t)__popc(w[0] & 0x11111111u) << 22, 0x00400000u);
     } else {
-        const uint32_t h = (w[1] >> 24) & 1u;
-        const uint32_t base = 0x60006000u | h | (h << 16);
-        const uint32_t hi = w[1] ^ ((uint32_t)__popc((w[0] ^ w[1]) & 0x01010101u) << 31 >> 7);
+        const uint32_t base = (spread<24>(w[1]) & 0x00010001u) | 0x60006000u;
+        const uint32_t hi = flip(w[1], (uint32_t)__popc((w[0] ^ w[1]) & 0x01010101u) << 24, 0x01000000u);
         // byte i of the low word and of the high word
         r[0] = (__builtin_amdgcn_perm(hi, w[0], 0x0c040c00u) << 1) | base;
         r[1] = (__builtin_amdgcn_perm(hi, w[0], 0x0c050c01u) << 1) | base;
@@ -183,7 +199,7 @@ __device__ __forceinline__ void value_pair(const uint32_t* a, const uint32_t* b,
         z += z << 8;
         z += z << 4;
         const uint32_t base = 0x4c004c00u | ((hi >> 7) & 0x00200020u);
-        const uint32_t fixed = hi ^ (z & 0x10001000u);
+        const uint32_t fixed = flip(hi, z, 0x10001000u);
         if constexpr (E == 8) {
             r[0] = nibbles<0>(lo, base);
             r[1] = nibbles<1>(lo, base);
@@ -202,8 +218,8 @@ __device__ __forceinline__ void value_pair(const uint32_t* a, const uint32_t* b,
         }
     } else {
         const uint32_t base = 0x60006000u | ((a[1] >> 24) & 1u) | ((b[1] >> 8) & 0x00010000u);
-        const uint32_t ha = a[1] ^ ((uint32_t)__popc((a[0] ^ a[1]) & 0x01010101u) << 31 >> 7);
-        const uint32_t hb = b[1] ^ ((uint32_t)__popc((b[0] ^ b[1]) & 0x01010101u) << 31 >> 7);
+        const uint32_t ha = flip(a[1], (uint32_t)__popc((a[0] ^ a[1]) & 0x01010101u) << 24, 0x01000000u);
+        const uint32_t hb = flip(b[1], (uint32_t)__popc((b[0] ^ b[1]) & 0x01010101u) << 24, 0x01000000u);
         const uint32_t la = E == 4 && upper ? ha : a[0], lb = E == 4 && upper ? hb : b[0];
         r[0] = (__builtin_amdgcn_perm(lb, la, 0x0c040c00u) << 1) | base;
         r[1] = (__builtin_amdgcn_perm(lb, la, 0x0c050c01u) << 1) | base;
@@ -503,13 +519,14 @@ struct Rows {
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) top = fmaxf(top, w[i]);
-                return top;
+                // a zero vector's scale is zero, which hides how large its e^s is
+                return fmaxf(top, sum * 0x1p-90f);
             };
             if (__any(attempt() > kDue)) {
                 float most = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float at = fmaf(s[i >> 2][r][i & 3], bk[i], __builtin_amdgcn_logf(bv[i]));
+                    const float at = fmaf(s[i >> 2][r][i & 3], bk[i], __builtin_amdgcn_logf(fmaxf(bv[i], 0x1p-70f)));
                     most = fmaxf(most, seen >> i & 1u ? at : -INFINITY);
                 }
                 const float to = fmaxf(M[r], over_groups_max(most) - kSettle);
@@ -659,17 +676,23 @@ __device__ __forceinline__ void leave(const Parts& parts, const KvAttentionArgs&
     parts.descs[id] = d;
 }
 
-// The cache row of a token (a multiple of 16) of sequence b's key head kh.
+// The cache row of a token (a multiple of 16) of sequence b's key head kh, in
+// two steps: the table's entry, which a loop reads a step ahead, and the row.
 struct Pages {
     ConstInts table;
     int kh;
     __device__ __forceinline__ Pages(const KvAttentionArgs& a, int b, int kh_) : table(constant(a.table + (int64_t)b * a.table_stride)), kh(kh_) {}
-    __device__ __forceinline__ int64_t row(const KvAttentionArgs& a, int token) const
+    __device__ __forceinline__ int entry(const KvAttentionArgs& a, int token) const
+    {
+        return table[min((int)u32div((uint32_t)token, a.c.page_div), a.max_pages - 1)];
+    }
+    __device__ __forceinline__ int64_t row(const KvAttentionArgs& a, int token, int entry) const
     {
         const uint32_t i = u32div((uint32_t)token, a.c.page_div);
-        const uint32_t page = min((uint32_t)max(table[min((int)i, a.max_pages - 1)], 0), a.c.pages - 1);
+        const uint32_t page = min((uint32_t)max(entry, 0), a.c.pages - 1);
         return ((int64_t)page * a.c.heads + kh) * a.c.page_size + (token - i * a.c.page_size);
     }
+    __device__ __forceinline__ int64_t row(const KvAttentionArgs& a, int token) const { return row(a, token, entry(a, token)); }
 };
 
 // The same value, but not one that the compiler can compute ahead of the
@@ -733,29 +756,35 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
         const Pages pages(a, ln.b, kh);
         int token = (ln.step * kWaves + wave) * kTile;
         const int stop = min((ln.step + count) * kStep, reach);
-        // one set of registers: the next keys are loaded behind the scores'
-        // product, the next values behind the second one, so that each has
-        // about half a step to arrive
+        // One set of registers: the next step's keys are loaded where this
+        // step's have been used, and so the scales and the values, each about
+        // half a step ahead (a second set, two steps ahead, was slower: 82 us
+        // for 79 on 64 sequences of 1000 to 8192 tokens).
         uint32_t kw[2][C * W], vw[2][T::B][4 * W], sc[2][4];
-        int64_t at[2];
+        // the step behind this one (the last one again); its second half if any of it is seen
+        auto ahead_of = [&](int t) { return t + kStep < stop ? t + kStep : t; };
+        auto half_of = [&](int t) { return t + 16 < reach ? t + 16 : t; };
+        int entry[2];
         R rs;
         typename R::Raw raw;
         rs.load(a, sq, kh, row0, here(lane), raw);
         if (token < stop) {
-            at[0] = pages.row(a, token);
-            at[1] = pages.row(a, token + 16 < reach ? token + 16 : token);
+            const int64_t at[2] = {pages.row(a, token), pages.row(a, half_of(token))};
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.keys(a.c, at[h], kw[h]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.scales(a.c, at[h], sc[h]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) words.values(a.c, at[h], vw[h]);
+            entry[0] = pages.entry(a, ahead_of(token));
+            entry[1] = pages.entry(a, half_of(ahead_of(token)));
         }
         const float factor = rs.convert(a, raw, R::top(a, raw, g), g);
         for (; token < stop; token += kStep) {
-            const int ahead = token + kStep < stop ? token + kStep : token;
-            at[0] = pages.row(a, ahead);
-            at[1] = pages.row(a, ahead + 16 < reach ? ahead + 16 : ahead);
+            const int ahead = ahead_of(token);
+            const int64_t at[2] = {pages.row(a, ahead, entry[0]), pages.row(a, half_of(ahead), entry[1])};
+            entry[0] = pages.entry(a, ahead_of(ahead));
+            entry[1] = pages.entry(a, half_of(ahead_of(ahead)));
             f32x4_kv s[2][NR];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -929,7 +958,7 @@ __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArg
 
         uint32_t kw[KC * W], vw[4 * W], sw;
         float factor = 0.f;
-        auto row_of = [&](int from) { return pages.row(a, from + 16 * sub < reach ? from + 16 * sub : from); };
+        auto place = [&](int from) { return from + 16 * sub < reach ? from + 16 * sub : from; };
         auto fetch = [&](int64_t row) {
             if (has_keys) {
                 const char* p = reinterpret_cast<const char*>(a.c.k) + row * row_bytes + k_at;
@@ -982,7 +1011,7 @@ __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArg
         R rs;
         typename R::Raw raw;
         rs.load(a, sq, kh, first, here(lane), raw);
-        if (token < stop) fetch(row_of(token));
+        if (token < stop) fetch(pages.row(a, place(token)));
         {
             const uint32_t t = R::top(a, raw, g);
             if (lane == 0) sh_top[wave] = t;
@@ -994,11 +1023,11 @@ __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArg
         }
         if (token < stop) {
             decode(0);
-            if (token + kSpan < stop) fetch(row_of(token + kSpan));
+            if (token + kSpan < stop) fetch(pages.row(a, place(token + kSpan)));
         }
+        int entry = token + 2 * kSpan < stop ? pages.entry(a, place(token + 2 * kSpan)) : 0;
         __syncthreads();
         for (int buf = 0; token < stop; token += kSpan, buf ^= 1) {
-            const int64_t beyond = row_of(min(token + 2 * kSpan, stop - 1) & ~15);
 #pragma unroll
             for (int p = 0; p < kSub / 2; ++p) {
                 const int at = token + kTile * p;
@@ -1029,7 +1058,8 @@ __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArg
             }
             if (token + kSpan < stop) {
                 decode(buf ^ 1);
-                if (token + 2 * kSpan < stop) fetch(beyond);
+                if (token + 2 * kSpan < stop) fetch(pages.row(a, place(token + 2 * kSpan), entry));
+                if (token + 3 * kSpan < stop) entry = pages.entry(a, place(token + 3 * kSpan));
             }
             __syncthreads();
         }
