@@ -42,6 +42,7 @@ namespace {
 typedef _Float16 half8_kv __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_kv __attribute__((ext_vector_type(2)));
 typedef float f32x4_kv __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2_kv __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_kv __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
@@ -314,6 +315,15 @@ __device__ __forceinline__ float over_groups_sum(float v)
     return v + __shfl_xor(v, 32, 64);
 }
 
+// The same value, but not one that the compiler can compute ahead of the
+// loops: what a segment's beginning and end derive from the lane would else be
+// kept in registers through the steps.
+__device__ __forceinline__ int here(int v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 __device__ __forceinline__ uint32_t ones(int n) { return n <= 0 ? 0u : n >= 4 ? 15u : (1u << n) - 1u; }
 
 // Which of the tokens place .. place + 3 a row sees: those below its limit
@@ -343,7 +353,7 @@ template <int DP, int BITS, int NR, int DT, bool QS, bool PS>
 struct Rows {
     static constexpr int C = DP / 32, NT = DP / 16;
     uint32_t q_hi[NR][C][4], q_lo[NR][QS ? C : 1][4];
-    float bias[NR];              // what the keys' offset adds to the scores, negated
+    f32x4_kv bias[NR];           // what the keys' offset adds to the scores, negated
     int limit[NR], own[NR];      // a row sees tokens below limit; own: its query token
     uint64_t drafts[NR];         // its row of the mask, the first word
     float M[NR], l[NR];
@@ -397,37 +407,57 @@ struct Rows {
         }
     }
 
-    // element j of a row's block c in fp32; zero past dim
-    __device__ __forceinline__ static float value(const KvAttentionArgs& a, const Raw& raw, int r, int c, int j, int g)
+    // elements 2 i and 2 i + 1 of a row's block c in fp32
+    __device__ __forceinline__ static void pair(const Raw& raw, int r, int c, int i, float& x, float& y)
     {
-        float x, y;
         if constexpr (DT == DT_F32) {
-            x = __uint_as_float(raw.x[r][c][j >> 2][j & 3]);
+            x = __uint_as_float(raw.x[r][c][i >> 1][2 * (i & 1)]);
+            y = __uint_as_float(raw.x[r][c][i >> 1][2 * (i & 1) + 1]);
         } else {
-            unpack2<DT>(raw.x[r][c][0][j >> 1], x, y);
-            if (j & 1) x = y;
+            unpack2<DT>(raw.x[r][c][0][i], x, y);
         }
-        return C * g + c < (a.c.dim >> 3) ? x : 0.f;
     }
 
-    // The largest finite row maximum, as bits, over the wave.
-    __device__ __forceinline__ static uint32_t top(const KvAttentionArgs& a, const Raw& raw, int g)
+    // Zeros past dim; returns the largest finite row maximum, as bits, over the wave.
+    __device__ __forceinline__ static uint32_t top(const KvAttentionArgs& a, Raw& raw, int g)
     {
         uint32_t most = 0;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
+            if (a.c.dim != DP) {
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int i = 0; i < kRaw; ++i)
+                        if (C * g + c >= (a.c.dim >> 3)) raw.x[r][c][i] = u32x4_kv{0u, 0u, 0u, 0u};
+            }
             uint32_t t = 0;
+            if constexpr (DT == DT_F32) {
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+                for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) t = max(t, __float_as_uint(value(a, raw, r, c, j, g)) & 0x7fffffffu);
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) t = max(t, raw.x[r][c][i][j] & 0x7fffffffu);
+            } else {
+                // magnitudes of 16 bits in order of their bits, two at a time
+                u16x2_kv m = {0, 0};
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_kv, raw.x[r][c][0][j] & 0x7fff7fffu));
+                float x, y;
+                unpack2<DT>((uint32_t)max(m.x, m.y), x, y);
+                t = __float_as_uint(x);
+            }
             t = max(t, (uint32_t)__shfl_xor((int)t, 16, 64));
             t = max(t, (uint32_t)__shfl_xor((int)t, 32, 64));
             most = max(most, t < 0x7f800000u ? t : 0u);
         }
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
-        return most;
+        return __builtin_amdgcn_readfirstlane(most);
     }
 
     // To fp16 times 2^k, which brings the workgroup's largest value (bits
@@ -435,26 +465,36 @@ struct Rows {
     // keys' scales.  What a small row loses is 2^-38 of the largest one in
     // absolute terms, far below the rounding of that one's scores.  Returns
     // what the scores are multiplied by.
-    __device__ __forceinline__ float convert(const KvAttentionArgs& a, const Raw& raw, uint32_t most, int g)
+    __device__ __forceinline__ float convert(const KvAttentionArgs& a, const Raw& raw, uint32_t most)
     {
         const int e = max((int)(most >> 23), 24);
         const float up = copysignf(__uint_as_float((uint32_t)(267 - e) << 23), a.scale);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            float sum = 0.f;
+            bias[r] = f32x4_kv{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < C; ++c) {
+                // elements i and i + 4 together
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pair(raw, r, c, i, x[2 * i], x[2 * i + 1]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float u = value(a, raw, r, c, i, g) * up, v = value(a, raw, r, c, i + 4, g) * up;
+                    const float u = x[i] * up, v = x[i + 4] * up;
                     q_hi[r][c][i] = pack2<DT_F16>(u, v);
-                    float hu, hv;
-                    unpack2<DT_F16>(q_hi[r][c][i], hu, hv);
-                    sum += hu + hv;
-                    if constexpr (QS) q_lo[r][c][i] = pack2<DT_F16>(u - hu, v - hv);
+                    if constexpr (QS) {
+                        float hu, hv;
+                        unpack2<DT_F16>(q_hi[r][c][i], hu, hv);
+                        q_lo[r][c][i] = pack2<DT_F16>(u - hu, v - hv);
+                    }
                 }
+                // the offset of every key times the row, negated
+                if constexpr (!QS)
+                    bias[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        __builtin_bit_cast(half8_kv, u32x4_kv{kBack<BITS>, kBack<BITS>, kBack<BITS>, kBack<BITS>}),
+                        __builtin_bit_cast(half8_kv, u32x4_kv{q_hi[r][c][0], q_hi[r][c][1], q_hi[r][c][2], q_hi[r][c][3]}),
+                        bias[r], 0, 0, 0);
             }
-            bias[r] = QS ? 0.f : -kOffset<BITS> * over_groups_sum(sum);
             M[r] = kNone;
             l[r] = 0.f;
 #pragma unroll
@@ -490,9 +530,11 @@ struct Rows {
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             uint32_t seen = 0xffu;
-            if (!whole)
-                seen = seen_of(a, sq, limit[r], own[r], drafts[r], token + 4 * g) |
-                       seen_of(a, sq, limit[r], own[r], drafts[r], token + 16 + 4 * g) << 4;
+            if (!whole) {
+                const int first = here(token + 4 * g);
+                seen = seen_of(a, sq, limit[r], own[r], drafts[r], first) |
+                       seen_of(a, sq, limit[r], own[r], drafts[r], first + 16) << 4;
+            }
             float w[8], sum;
             // a second time where the reference M had to move (and no third,
             // whatever the scores)
@@ -695,15 +737,6 @@ struct Pages {
     __device__ __forceinline__ int64_t row(const KvAttentionArgs& a, int token) const { return row(a, token, entry(a, token)); }
 };
 
-// The same value, but not one that the compiler can compute ahead of the
-// loops: what a segment's beginning and end derive from the lane would else be
-// kept in registers through the steps.
-__device__ __forceinline__ int here(int v)
-{
-    asm volatile("" : "+v"(v));
-    return v;
-}
-
 __device__ __forceinline__ int xcd_id()
 {
     // neighbouring runs on one XCD (workgroups go to the 8 XCDs in turn)
@@ -779,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
             entry[0] = pages.entry(a, ahead_of(token));
             entry[1] = pages.entry(a, half_of(ahead_of(token)));
         }
-        const float factor = rs.convert(a, raw, R::top(a, raw, g), g);
+        const float factor = rs.convert(a, raw, R::top(a, raw, g));
         for (; token < stop; token += kStep) {
             const int ahead = ahead_of(token);
             const int64_t at[2] = {pages.row(a, ahead, entry[0]), pages.row(a, half_of(ahead), entry[1])};
@@ -789,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int r = 0; r < NR; ++r) s[h][r] = f32x4_kv{rs.bias[r], rs.bias[r], rs.bias[r], rs.bias[r]};
+                for (int r = 0; r < NR; ++r) s[h][r] = rs.bias[r];
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     uint32_t k[4];
@@ -956,6 +989,13 @@ __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArg
         int token = ln.step * kSpan;
         const int stop = min((ln.step + count) * kSpan, reach);
 
+        // A vector load issued before the words': the scalar one would be
+        // waited for together with all LDS writes.
+        int entry = 0;
+        auto entry_of = [&](int t) {
+            const int i = min((int)u32div((uint32_t)t, a.c.page_div), a.max_pages - 1);
+            return a.table[(int64_t)ln.b * a.table_stride + here(i)];
+        };
         uint32_t kw[KC * W], vw[4 * W], sw;
         float factor = 0.f;
         auto place = [&](int from) { return from + 16 * sub < reach ? from + 16 * sub : from; };
@@ -1019,13 +1059,16 @@ __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArg
             uint32_t most = sh_top[0];
 #pragma unroll
             for (int w = 1; w < WAVES; ++w) most = max(most, sh_top[w]);
-            factor = rs.convert(a, raw, most, g);
+            factor = rs.convert(a, raw, most);
         }
         if (token < stop) {
             decode(0);
-            if (token + kSpan < stop) fetch(pages.row(a, place(token + kSpan)));
+            if (token + kSpan < stop) {
+                const int64_t row = pages.row(a, place(token + kSpan));
+                if (token + 2 * kSpan < stop) entry = entry_of(place(token + 2 * kSpan));
+                fetch(row);
+            }
         }
-        int entry = token + 2 * kSpan < stop ? pages.entry(a, place(token + 2 * kSpan)) : 0;
         __syncthreads();
         for (int buf = 0; token < stop; token += kSpan, buf ^= 1) {
 #pragma unroll
@@ -1036,7 +1079,7 @@ __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArg
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) s[h][r] = f32x4_kv{rs.bias[r], rs.bias[r], rs.bias[r], rs.bias[r]};
+                    for (int r = 0; r < NR; ++r) s[h][r] = rs.bias[r];
 #pragma unroll
                     for (int c = 0; c < C; ++c) rs.score(s[h], sh_k[buf][2 * p + h][c][lane], c);
                 }
@@ -1051,15 +1094,27 @@ __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArg
                         bv[4 * h + j] = y[j];
                     }
                 }
+                // the values' operands under way while the weights are computed, where there are registers for them
+                // (two tiles a wave with them: 88 us for 78 on trees of 32 drafted tokens)
+                constexpr int kEarly = NR == 1 ? NT : 0;
+                u32x4_kv vf[NT];
+#pragma unroll
+                for (int j = 0; j < kEarly; ++j) vf[j] = sh_v[buf][p][j][lane];
                 uint32_t p_hi[NR][4], p_lo[NR][4];
                 rs.weigh(a, sq, s, bk, bv, at, at + kTile <= all, g, p_hi, p_lo);
 #pragma unroll
-                for (int j = 0; j < NT; ++j) rs.add(sh_v[buf][p][j][lane], j, p_hi, p_lo);
+                for (int j = 0; j < NT; ++j) {
+                    if (j >= kEarly) vf[j] = sh_v[buf][p][j][lane];
+                    rs.add(vf[j], j, p_hi, p_lo);
+                }
             }
             if (token + kSpan < stop) {
                 decode(buf ^ 1);
-                if (token + 2 * kSpan < stop) fetch(pages.row(a, place(token + 2 * kSpan), entry));
-                if (token + 3 * kSpan < stop) entry = pages.entry(a, place(token + 3 * kSpan));
+                if (token + 2 * kSpan < stop) {
+                    const int64_t row = pages.row(a, place(token + 2 * kSpan), __builtin_amdgcn_readfirstlane(entry));
+                    if (token + 3 * kSpan < stop) entry = entry_of(place(token + 3 * kSpan));
+                    fetch(row);
+                }
             }
             __syncthreads();
         }
@@ -1153,6 +1208,38 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(KvAttentionArgs a, in
     if (a.lse && across == 0) a.lse[at] = some ? (m + log2f(l)) * (1.f / kLog2e) : -INFINITY;
 }
 
+// The same where a tile has many rows (and few parts): DP / 4 threads across a
+// row, which go through its parts in order.
+template <int DP, int ROWS, int DT>
+__global__ void __launch_bounds__(kThreads) kv_join_rows_kernel(KvAttentionArgs a, int blocks)
+{
+    constexpr int kAcross = DP / 4, kAtOnce = kThreads / kAcross;
+    const Desc d = reinterpret_cast<const Desc*>(a.workspace)[blockIdx.x];
+    const int across = threadIdx.x % kAcross, row = blockIdx.y * kAtOnce + threadIdx.x / kAcross;
+    if (d.parts == 0 || row >= d.rows) return;
+    const Parts parts(a.workspace, blocks, ROWS);
+    auto slot = [&](int p) { return (int64_t)(2 * ((int)blockIdx.x + p) + (p == 0 ? 1 : 0)) * ROWS + row; };
+    float m = kNone;
+    for (int p = 0; p < d.parts; ++p) m = fmaxf(m, parts.ml[slot(p) * 2]);
+    f32x4_kv o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    if (4 * across >= a.c.dim) return;
+#pragma unroll 2
+    for (int p = 0; p < d.parts; ++p) {
+        const int64_t at = slot(p);
+        const float f = __builtin_amdgcn_exp2f(parts.ml[at * 2] - m);
+        l += parts.ml[at * 2 + 1] * f;
+        o += *reinterpret_cast<const f32x4_kv*>(parts.o + at * DP + 4 * across) * f;
+    }
+    const bool some = l > 0.f || l != l;
+    const float inv = some ? 1.f / l : 0.f;
+    const uint32_t t = u32div((uint32_t)(d.row0 + row), a.group_div);
+    const int64_t at = ((int64_t)d.token0 + t) * a.heads + d.head * a.group + (d.row0 + row - (int)t * a.group);
+    const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    store_n<DT, 4>(a.out, at * a.c.dim + 4 * across, x);
+    if (a.lse && across == 0) a.lse[at] = some ? (m + log2f(l)) * (1.f / kLog2e) : -INFINITY;
+}
+
 template <int DP, int BITS, int NR, int WAVES, int DT>
 hipError_t launch(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_t s)
 {
@@ -1171,8 +1258,14 @@ hipError_t launch(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_
     if (e != hipSuccess || most_parts <= 1) return e;
     // rows of a tile that can be in use
     const int64_t rows = a.starts ? a.n * a.group : a.n / a.seqs * a.group;
-    hipLaunchKernelGGL((kv_join_kernel<DP, kRows, DT>), dim3(p.blocks, (unsigned)(rows < kRows ? rows : kRows)),
-                       dim3(kThreads), 0, s, a, p.blocks);
+    const int used = (int)(rows < kRows ? rows : kRows);
+    if constexpr (kMany) {
+        constexpr int kAtOnce = kThreads / (DP / 4);
+        hipLaunchKernelGGL((kv_join_rows_kernel<DP, kRows, DT>), dim3(p.blocks, (used + kAtOnce - 1) / kAtOnce),
+                           dim3(kThreads), 0, s, a, p.blocks);
+    } else {
+        hipLaunchKernelGGL((kv_join_kernel<DP, kRows, DT>), dim3(p.blocks, used), dim3(kThreads), 0, s, a, p.blocks);
+    }
     return hipGetLastError();
 }
 
