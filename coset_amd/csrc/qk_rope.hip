@@ -12,8 +12,8 @@
 //
 // A lane holds 8 values of a head: both halves of 4 pairs (two 4-value loads
 // rot/2 apart, or 8 neighbours interleaved), or 8 values behind the rotated
-// part, so no value crosses lanes but in the norm's sums.  The dim / 8 lanes
-// of a token keep its cosines and sines in registers and walk over heads.
+// part, so no value crosses lanes but in the norm's sums.  The lanes of a token
+// keep what its angles make of the weights in registers and walk over heads.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -25,7 +25,8 @@ namespace coset {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxGroups = 512;   // backward: workgroups along the tokens, one row of weight sums each
+constexpr int kMaxForward = 1024; // forward: workgroups
+constexpr int kMaxGroups = 1024;   // backward: workgroups, one row of weight sums each
 
 struct Lane {
     int first, second;   // element of x[0..3] and of x[4..7]
@@ -53,6 +54,51 @@ __device__ __forceinline__ void load8(const void* p, int64_t at, const Lane& l, 
     load_n<DT, 4>(p, at + l.second, vec, x + 4);
 }
 
+// The same, still in the input's type: 16-bit values two a register.
+template <int DT>
+struct Raw {
+    uint32_t u[DT == DT_F32 ? 8 : 4];
+
+    __device__ __forceinline__ void load(const void* p, int64_t at, const Lane& l, bool vec)
+    {
+        if constexpr (DT == DT_F32) {
+            float x[8];
+            load8<DT>(p, at, l, vec, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(x[j]);
+        } else {
+            const uint16_t* f = reinterpret_cast<const uint16_t*>(p) + at + l.first;
+            const uint16_t* b = reinterpret_cast<const uint16_t*>(p) + at + l.second;
+            if (vec) {
+                const uint2 v = *reinterpret_cast<const uint2*>(f), w = *reinterpret_cast<const uint2*>(b);
+                u[0] = v.x;
+                u[1] = v.y;
+                u[2] = w.x;
+                u[3] = w.y;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    u[j] = (uint32_t)f[2 * j] | (uint32_t)f[2 * j + 1] << 16;
+                    u[2 + j] = (uint32_t)b[2 * j] | (uint32_t)b[2 * j + 1] << 16;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void values(float (&x)[8]) const
+    {
+        if constexpr (DT == DT_F32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(u[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) unpack2<DT>(u[j], x[2 * j], x[2 * j + 1]);
+        }
+    }
+};
+
+// Loads under way a lane: this many heads' while as many are computed.
+constexpr int kAhead = 4;
+
 template <int DT>
 __device__ __forceinline__ void store8(void* p, int64_t at, const Lane& l, const float (&x)[8])
 {
@@ -60,16 +106,23 @@ __device__ __forceinline__ void store8(void* p, int64_t at, const Lane& l, const
     store_n<DT, 4>(p, at + l.second, x + 4);
 }
 
+template <int DT>
+__device__ __forceinline__ void weight_as(const void* w, const Lane& l, float (&x)[8])
+{
+    load8<DT>(w, 0, l, (reinterpret_cast<uintptr_t>(w) & 15) == 0, x);
+}
+
 __device__ __forceinline__ void load_weight(const void* w, int dt, const Lane& l, float (&x)[8])
 {
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = 1.f;
     if (!w || !l.on) return;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int e = j < 4 ? l.first + j : l.second + j - 4;
-        x[j] = dt == DT_F32 ? load1<DT_F32>(w, e) : dt == DT_BF16 ? load1<DT_BF16>(w, e) : load1<DT_F16>(w, e);
-    }
+    if (dt == DT_F32)
+        weight_as<DT_F32>(w, l, x);
+    else if (dt == DT_BF16)
+        weight_as<DT_BF16>(w, l, x);
+    else
+        weight_as<DT_F16>(w, l, x);
 }
 
 // cosines and sines of the lane's four pairs 4l..4l+3
@@ -82,8 +135,14 @@ __device__ __forceinline__ void load_turn(const RopeArgs& a, int l, int64_t t, c
     }
     if (!ln.turned) return;
     const int half = a.rot / 2;
-    if (a.axes == 1) {
-        const int64_t p = min(max(a.pos[t], (int64_t)0), a.length - 1);
+    // the four pairs' axis, where they have one
+    int first = 0, last = 0;
+    for (int k = 0; k + 1 < a.axes; ++k) {
+        first += 4 * l >= a.bound[k] ? 1 : 0;
+        last += 4 * l + 3 >= a.bound[k] ? 1 : 0;
+    }
+    if (first == last) {
+        const int64_t p = min(max(a.pos[first * a.pos_axis + t], (int64_t)0), a.length - 1);
         const float4 cc = *reinterpret_cast<const float4*>(a.table + p * a.rot + 4 * l);
         const float4 ss = *reinterpret_cast<const float4*>(a.table + p * a.rot + half + 4 * l);
         c[0] = cc.x;
@@ -107,118 +166,194 @@ __device__ __forceinline__ void load_turn(const RopeArgs& a, int l, int64_t t, c
     }
 }
 
-// (x_a, x_b) turned by +-angle; pairs (x[i], x[4+i]) or (x[2i], x[2i+1])
-__device__ __forceinline__ void turn(float (&x)[8], const float (&c)[4], const float (&s)[4], bool near, float sign)
+// Sum over the GW lanes of a group, in every lane: within rows of 16 lanes by
+// data-parallel moves, beyond by the LDS crossbar.
+template <int CTRL>
+__device__ __forceinline__ float moved(float v)
 {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float u = near ? x[2 * i] : x[i], v = near ? x[2 * i + 1] : x[4 + i];
-        const float si = sign * s[i];
-        const float y = u * c[i] - v * si, z = v * c[i] + u * si;
-        if (near) {
-            x[2 * i] = y;
-            x[2 * i + 1] = z;
-        } else {
-            x[i] = y;
-            x[4 + i] = z;
-        }
-    }
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
 }
-
 template <int GW>
 __device__ __forceinline__ float group_sum(float v)
 {
-#pragma unroll
-    for (int o = 1; o < GW; o <<= 1) v += __shfl_xor(v, o, 64);
+    v += moved<0xb1>(v);                              // lane ^ 1
+    v += moved<0x4e>(v);                              // lane ^ 2
+    if constexpr (GW >= 8) v += moved<0x141>(v);      // the other four of eight (mirrored)
+    if constexpr (GW >= 16) v += moved<0x140>(v);     // the other eight of sixteen (mirrored)
+    if constexpr (GW >= 32) v += __shfl_xor(v, 16, 64);
+    if constexpr (GW >= 64) v += __shfl_xor(v, 32, 64);
     return v;
 }
 
-// Heads [h0, h1) of the queries followed by the keys.
+// places of pair i's two values among a lane's eight
+template <bool NEAR>
+__device__ __forceinline__ constexpr int front(int i) { return NEAR ? 2 * i : i; }
+template <bool NEAR>
+__device__ __forceinline__ constexpr int back(int i) { return NEAR ? 2 * i + 1 : i + 4; }
+
+// One side's heads [h0, h1) of token t.  y_a = r (x_a (w_a cos) - x_b (w_b sin)):
+// the weights' products with the angle are the token's, not the head's.
+template <int DT, int GW, bool NEAR>
+__device__ __forceinline__ void forward_side(const RopeArgs& a, const RopeSide& sd, int64_t t, int h0, int h1, const Lane& ln,
+                                             const float (&w)[8], const float (&c)[4], const float (&s)[4])
+{
+    if (h0 >= h1) return;
+    float ac[4], bs[4], bc[4], as[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float wa = w[front<NEAR>(i)], wb = w[back<NEAR>(i)];
+        ac[i] = wa * c[i];
+        as[i] = wa * s[i];
+        bc[i] = wb * c[i];
+        bs[i] = wb * s[i];
+    }
+    const float mean = 1.f / (float)a.dim;
+    const int64_t at = t * sd.x_tok;
+    int64_t out = (t * sd.heads + h0) * (int64_t)a.dim;
+    Raw<DT> next[kAhead] = {};
+    auto fetch = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (ln.on && h + i < h1) next[i].load(sd.x, at + (h + i) * sd.x_head, ln, sd.vec);
+    };
+    fetch(h0);
+    for (int h = h0; h < h1; h += kAhead) {
+        Raw<DT> raw[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) raw[i] = next[i];
+        fetch(h + kAhead);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (h + k >= h1) break;
+            float x[8], y[8];
+            raw[k].values(x);
+            float r = 1.f;
+            if (a.norm) {
+                float sq = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sq = fmaf(x[j], x[j], sq);
+                r = __builtin_amdgcn_rsqf(fmaf(group_sum<GW>(sq), mean, a.eps));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = x[front<NEAR>(i)], v = x[back<NEAR>(i)];
+                y[front<NEAR>(i)] = r * fmaf(u, ac[i], -(v * bs[i]));
+                y[back<NEAR>(i)] = r * fmaf(v, bc[i], u * as[i]);
+            }
+            if (ln.on) store8<DT>(sd.out, out, ln, y);
+            out += a.dim;
+        }
+    }
+}
+
+// The lanes of a group take a token and walk over its heads [h0, h1) of the
+// queries followed by the keys.
 template <int DT, int GW, bool NEAR>
 __global__ void __launch_bounds__(kThreads) rope_fwd_kernel(RopeArgs a, int per)
 {
+    constexpr int kTokens = kThreads / GW;
     const int l = threadIdx.x % GW;
-    const int64_t t = (int64_t)blockIdx.x * (kThreads / GW) + threadIdx.x / GW;
-    if (t >= a.n) return;
     const Lane ln = lane_of(a, l);
-    float c[4], s[4], wq[8], wk[8];
-    load_turn(a, l, t, ln, c, s);
+    float wq[8], wk[8];
     load_weight(a.q.w, a.w_dtype, ln, wq);
     load_weight(a.k.w, a.w_dtype, ln, wk);
     const int h0 = blockIdx.y * per, h1 = min(h0 + per, a.q.heads + a.k.heads);
-    const float mean = 1.f / (float)a.dim;
-    for (int h = h0; h < h1; ++h) {
-        const bool key = h >= a.q.heads;
-        const RopeSide& sd = key ? a.k : a.q;
-        const int hh = key ? h - a.q.heads : h;
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (ln.on) load8<DT>(sd.x, t * sd.x_tok + hh * sd.x_head, ln, sd.vec, x);
-        if (a.norm) {
-            float sq = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sq = fmaf(x[j], x[j], sq);
-            const float r = 1.f / sqrtf(fmaf(group_sum<GW>(sq), mean, a.eps));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = x[j] * r * (key ? wk[j] : wq[j]);
-        }
-        turn(x, c, s, NEAR, 1.f);
-        if (ln.on) store8<DT>(sd.out, (t * sd.heads + hh) * (int64_t)a.dim, ln, x);
+    for (int64_t t = (int64_t)blockIdx.x * kTokens + threadIdx.x / GW; t < a.n; t += (int64_t)gridDim.x * kTokens) {
+        float c[4], s[4];
+        load_turn(a, l, t, ln, c, s);
+        forward_side<DT, GW, NEAR>(a, a.q, t, h0, min(h1, a.q.heads), ln, wq, c, s);
+        forward_side<DT, GW, NEAR>(a, a.k, t, max(h0 - a.q.heads, 0), h1 - a.q.heads, ln, wk, c, s);
     }
 }
 
 template <int DT, int GW, bool NEAR>
-__global__ void __launch_bounds__(kThreads) rope_bwd_kernel(RopeArgs a)
+__device__ __forceinline__ void backward_side(const RopeArgs& a, const RopeSide& sd, int64_t t, int h0, int h1, const Lane& ln,
+                                              const float (&w)[8], const float (&c)[4], const float (&s)[4], float (&dw)[8])
 {
-    constexpr int kTokens = kThreads / GW;
-    const int l = threadIdx.x % GW;
+    if (h0 >= h1) return;
+    const float mean = 1.f / (float)a.dim;
+    const int64_t xat = t * sd.x_tok, gat = t * sd.g_tok;
+    int64_t out = (t * sd.heads + h0) * (int64_t)a.dim;
+    constexpr int kBoth = kAhead / 2;
+    Raw<DT> xn[kBoth] = {}, gn[kBoth] = {};
+    auto fetch = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < kBoth; ++i)
+            if (ln.on && h + i < h1) {
+                gn[i].load(sd.g, gat + (h + i) * sd.g_head, ln, sd.vec);
+                if (a.norm) xn[i].load(sd.x, xat + (h + i) * sd.x_head, ln, sd.vec);
+            }
+    };
+    fetch(h0);
+    for (int h = h0; h < h1; h += kBoth) {
+        Raw<DT> xr[kBoth], gr[kBoth];
+#pragma unroll
+        for (int i = 0; i < kBoth; ++i) {
+            xr[i] = xn[i];
+            gr[i] = gn[i];
+        }
+        fetch(h + kBoth);
+#pragma unroll
+        for (int k = 0; k < kBoth; ++k) {
+            if (h + k >= h1) break;
+            float x[8], z[8], y[8];
+            xr[k].values(x);
+            gr[k].values(y);
+            // dz: the gradient turned back
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = y[front<NEAR>(i)], v = y[back<NEAR>(i)];
+                z[front<NEAR>(i)] = fmaf(u, c[i], v * s[i]);
+                z[back<NEAR>(i)] = fmaf(v, c[i], -(u * s[i]));
+            }
+            if (a.norm) {
+                float sq = 0.f, dot = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    sq = fmaf(x[j], x[j], sq);
+                    y[j] = z[j] * w[j];              // du
+                    dot = fmaf(y[j], x[j], dot);
+                }
+                const float r = __builtin_amdgcn_rsqf(fmaf(group_sum<GW>(sq), mean, a.eps));
+                const float m = group_sum<GW>(dot) * r * mean * r;   // r mean(du u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float u = x[j] * r;
+                    dw[j] = fmaf(z[j], u, dw[j]);
+                    y[j] = fmaf(-u, m, y[j] * r);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = z[j];
+            }
+            if (ln.on) store8<DT>(sd.out, out, ln, y);
+            out += a.dim;
+        }
+    }
+}
+
+template <int DT, int GW, bool NEAR>
+__global__ void __launch_bounds__(kThreads) rope_bwd_kernel(RopeArgs a, int per)
+{
+    constexpr int kGroups = kThreads / GW;
+    const int l = threadIdx.x % GW, group = threadIdx.x / GW;
     const Lane ln = lane_of(a, l);
     float wq[8], wk[8], dq[8], dk[8];
     load_weight(a.q.w, a.w_dtype, ln, wq);
     load_weight(a.k.w, a.w_dtype, ln, wk);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dq[j] = dk[j] = 0.f;
-    const float mean = 1.f / (float)a.dim;
-    for (int64_t t = (int64_t)blockIdx.x * kTokens + threadIdx.x / GW; t < a.n; t += (int64_t)gridDim.x * kTokens) {
+    const int h0 = blockIdx.y * per, h1 = min(h0 + per, a.q.heads + a.k.heads);
+    for (int64_t t = (int64_t)blockIdx.x * kGroups + group; t < a.n; t += (int64_t)gridDim.x * kGroups) {
         float c[4], s[4];
         load_turn(a, l, t, ln, c, s);
-        for (int h = 0; h < a.q.heads + a.k.heads; ++h) {
-            const bool key = h >= a.q.heads;
-            const RopeSide& sd = key ? a.k : a.q;
-            const int hh = key ? h - a.q.heads : h;
-            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, g[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (ln.on) {
-                load8<DT>(sd.g, t * sd.g_tok + hh * sd.g_head, ln, sd.vec, g);
-                if (a.norm) load8<DT>(sd.x, t * sd.x_tok + hh * sd.x_head, ln, sd.vec, x);
-            }
-            turn(g, c, s, NEAR, -1.f);
-            if (a.norm) {
-                float sq = 0.f, du[8], dot = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    sq = fmaf(x[j], x[j], sq);
-                    du[j] = g[j] * (key ? wk[j] : wq[j]);
-                    dot = fmaf(du[j], x[j], dot);
-                }
-                const float r = 1.f / sqrtf(fmaf(group_sum<GW>(sq), mean, a.eps));
-                const float m = group_sum<GW>(dot) * r * mean;   // mean(du u)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float u = x[j] * r;
-                    const float add = g[j] * u;
-                    if (key)
-                        dk[j] += add;
-                    else
-                        dq[j] += add;
-                    g[j] = r * fmaf(-u, m, du[j]);
-                }
-            }
-            if (ln.on) store8<DT>(sd.out, (t * sd.heads + hh) * (int64_t)a.dim, ln, g);
-        }
+        backward_side<DT, GW, NEAR>(a, a.q, t, h0, min(h1, a.q.heads), ln, wq, c, s, dq);
+        backward_side<DT, GW, NEAR>(a, a.k, t, max(h0 - a.q.heads, 0), h1 - a.q.heads, ln, wk, c, s, dk);
     }
     if (!a.partial) return;
-    // the workgroup's tokens in a fixed order
-    __shared__ float sh[2][kTokens][GW * 8];
-    const int row = threadIdx.x / GW;
+    // the workgroup's lane groups in a fixed order
+    __shared__ float sh[2][kGroups][GW * 8];
+    const int row = group;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         sh[0][row][j * GW + l] = dq[j];
@@ -228,10 +363,10 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(RopeArgs a)
     for (int i = threadIdx.x; i < 2 * GW * 8; i += kThreads) {
         const int side = i / (GW * 8), e = i % (GW * 8);
         float v = 0.f;
-        for (int r = 0; r < kTokens; ++r) v += sh[side][r][e];
+        for (int r = 0; r < kGroups; ++r) v += sh[side][r][e];
         const Lane le = lane_of(a, e % GW);
         const int j = e / GW;
-        if (le.on) a.partial[((int64_t)blockIdx.x * 2 + side) * a.dim + (j < 4 ? le.first + j : le.second + j - 4)] = v;
+        if (le.on) a.partial[((int64_t)(blockIdx.y * gridDim.x + blockIdx.x) * 2 + side) * a.dim + (j < 4 ? le.first + j : le.second + j - 4)] = v;
     }
 }
 
@@ -245,51 +380,69 @@ __device__ __forceinline__ void store_any(void* p, int dt, int64_t i, float v)
         store1<DT_F16>(p, i, v);
 }
 
-// The weights' gradients: 16 columns a workgroup, 16 threads of partials
+// The weights' gradients: 16 columns a workgroup, 64 threads of partials
 // each, summed in a fixed order.
-__global__ void __launch_bounds__(kThreads) rope_weight_kernel(RopeArgs a, int groups)
+__global__ void __launch_bounds__(1024) rope_weight_kernel(RopeArgs a, int groups)
 {
-    __shared__ float sh[16][17];
+    __shared__ float sh[64][17];
     const int col = threadIdx.x % 16, part = threadIdx.x / 16;
     const int e = blockIdx.x * 16 + col;
     const int side = blockIdx.y;
     float v = 0.f;
-    if (e < a.dim)
-        for (int g = part; g < groups; g += 16) v += a.partial[((int64_t)g * 2 + side) * a.dim + e];
+    if (e < a.dim) {
+#pragma unroll 4
+        for (int g = part; g < groups; g += 64) v += a.partial[((int64_t)g * 2 + side) * a.dim + e];
+    }
     sh[part][col] = v;
     __syncthreads();
     if (part == 0 && e < a.dim) {
         float t = 0.f;
-        for (int p = 0; p < 16; ++p) t += sh[p][col];
+#pragma unroll 8
+        for (int p = 0; p < 64; ++p) t += sh[p][col];
         void* out = side ? a.gw_k : a.gw_q;   // either may be unwanted
         if (out) store_any(out, a.w_dtype, e, t);
     }
 }
 
+// Workgroups along the tokens and along the heads: all heads of a lane group's
+// tokens where the tokens alone fill the chip (`most` workgroups), else the
+// heads are shared out too.
+struct Shape {
+    int across, shares, per;
+};
+Shape shape_of(const RopeArgs& a, int lanes, int most)
+{
+    const int heads = a.q.heads + a.k.heads;
+    const int64_t rows = (a.n + kThreads / lanes - 1) / (kThreads / lanes);
+    Shape g{};
+    g.across = (int)(rows < most ? rows : most);
+    int shares = 1;
+    while (g.across > 0 && 2 * shares * g.across <= most && shares < heads) shares *= 2;
+    g.per = (heads + shares - 1) / shares;
+    g.shares = (heads + g.per - 1) / g.per;
+    return g;
+}
+
 template <int DT, int GW, bool NEAR>
 hipError_t launch_fwd(const RopeArgs& a, hipStream_t s)
 {
-    const int heads = a.q.heads + a.k.heads;
-    const int64_t rows = (a.n + kThreads / GW - 1) / (kThreads / GW);
-    // one head a lane group until the grid holds 8 workgroups per CU
-    int per = 1;
-    while (per < heads && rows * ((heads + 2 * per - 1) / (2 * per)) >= 2048) per *= 2;
-    hipLaunchKernelGGL((rope_fwd_kernel<DT, GW, NEAR>), dim3((unsigned)rows, (heads + per - 1) / per), dim3(kThreads), 0,
-                       s, a, per);
+    const Shape g = shape_of(a, GW, kMaxForward);
+    hipLaunchKernelGGL((rope_fwd_kernel<DT, GW, NEAR>), dim3(g.across, g.shares), dim3(kThreads), 0, s, a, g.per);
     return hipGetLastError();
 }
 
 template <int DT, int GW, bool NEAR>
 hipError_t launch_bwd(const RopeArgs& a, hipStream_t s)
 {
-    const int groups = rope_bwd_groups(a.n, a.dim);
+    const Shape g = shape_of(a, GW, kMaxGroups);
+    const int groups = g.across * g.shares;
     hipError_t e = hipSuccess;
     if (groups > 0) {
-        hipLaunchKernelGGL((rope_bwd_kernel<DT, GW, NEAR>), dim3(groups), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL((rope_bwd_kernel<DT, GW, NEAR>), dim3(g.across, g.shares), dim3(kThreads), 0, s, a, g.per);
         e = hipGetLastError();
     }
     if (e != hipSuccess || (!a.gw_q && !a.gw_k)) return e;
-    hipLaunchKernelGGL(rope_weight_kernel, dim3((a.dim + 15) / 16, 2), dim3(kThreads), 0, s, a, groups);
+    hipLaunchKernelGGL(rope_weight_kernel, dim3((a.dim + 15) / 16, 2), dim3(1024), 0, s, a, groups);
     return hipGetLastError();
 }
 
@@ -324,11 +477,8 @@ hipError_t by_type(const RopeArgs& a, hipStream_t s)
 
 }  // namespace
 
-int rope_bwd_groups(int64_t n, int dim)
-{
-    const int64_t rows = (n + kThreads / lanes_of(dim) - 1) / (kThreads / lanes_of(dim));
-    return (int)(rows < kMaxGroups ? rows : kMaxGroups);
-}
+// Rows of weight sums at most.
+int rope_bwd_groups(int64_t n, int dim) { return n > 0 ? kMaxGroups : 0; }
 
 hipError_t launch_rope_fwd(const RopeArgs& a, hipStream_t s) { return a.n == 0 ? hipSuccess : by_type<false>(a, s); }
 hipError_t launch_rope_bwd(const RopeArgs& a, hipStream_t s) { return by_type<true>(a, s); }
