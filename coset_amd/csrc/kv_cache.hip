@@ -1,11 +1,11 @@
 // kv_cache.hip -- rows of the E8 key/value cache written and read back
 // (format and nearest-point rule: kv_cache.hpp).
 //
-// One lane holds one block of 8 coordinates; the 4 to 32 lanes of a vector
-// find its largest magnitude with butterflies.  A workgroup takes one head of
-// the keys or the values (blockIdx.y) and 256 / lanes-per-vector tokens, so
-// that the values' words of four neighbouring tokens, 16 bytes, leave in the
-// same store instruction.
+// A lane holds one or two blocks of 8 coordinates; the lanes of a vector find
+// its largest magnitude with data-parallel moves.  A workgroup takes one head
+// of the keys or the values (blockIdx.y) and neighbouring tokens, so that the
+// values' words of four of them, 16 bytes, leave in the same store
+// instruction.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -28,84 +28,132 @@ __device__ __forceinline__ int64_t kv_word(const KvCache& c, bool value, int64_t
     return value ? page + ((int64_t)((off >> 2) * nb + b) * 4 + (off & 3)) * W : page + ((int64_t)off * nb + b) * W;
 }
 
+// Over the GW lanes of a group, in every lane.
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t v)
+{
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int GW>
+__device__ __forceinline__ uint32_t group_max(uint32_t v)
+{
+    v = max(v, moved<0xb1>(v));                           // lane ^ 1
+    if constexpr (GW >= 4) v = max(v, moved<0x4e>(v));    // lane ^ 2
+    if constexpr (GW >= 8) v = max(v, moved<0x141>(v));   // the other four of eight (mirrored)
+    if constexpr (GW >= 16) v = max(v, moved<0x140>(v));  // the other eight of sixteen (mirrored)
+    return v;
+}
+
+// A lane writes two neighbouring blocks.
 template <int BITS, int DT, int GW>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(KvRowsArgs a)
 {
+    constexpr int W = BITS / 4;
     const int lane = threadIdx.x % GW;
     const int64_t t = (int64_t)blockIdx.x * (kThreads / GW) + threadIdx.x / GW;
     const bool value = blockIdx.y & 1;
     const uint32_t head = blockIdx.y >> 1;
     const int nb = a.c.dim >> 3;
-    const bool mine = t < a.n && lane < nb;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const bool mine = t < a.n && 2 * lane < nb;
+    float x[2][8] = {};
     int64_t slot = -1;
     if (mine) {
         slot = a.slots[t];
-        const int64_t at = t * (value ? a.v_tok : a.k_tok) + head * (value ? a.v_head : a.k_head) + 8 * lane;
-        load_n<DT, 8>(value ? a.v : a.k, at, a.vec, x);
+        const int64_t at = t * (value ? a.v_tok : a.k_tok) + head * (value ? a.v_head : a.k_head) + 16 * lane;
+        load_n<DT, 8>(value ? a.v : a.k, at, a.vec, x[0]);
+        load_n<DT, 8>(value ? a.v : a.k, at + 8, a.vec, x[1]);
     }
     // the largest magnitude as bits: a NaN is above infinity there
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 1; o < GW; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-    uint32_t scale = kv_scale_bits<BITS>(__uint_as_float(top));
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i >> 3][i & 7]) & 0x7fffffffu);
+    top = group_max<GW>(top);
+    const uint32_t scale = kv_scale_bits<BITS>(__uint_as_float(top));
     float beta = __uint_as_float(scale << 16);
     const bool fine = beta > 0.f;   // neither zero nor NaN
     if (!fine) {
         beta = 1.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+        for (int i = 0; i < 16; ++i) x[i >> 3][i & 7] = 0.f;
     }
-    uint32_t w[BITS / 4];
-    kv_nearest<BITS>(x, beta, __fdiv_rn(1.f, beta), w);
+    // one step corrects a reciprocal that is off by an ulp, two need it correctly rounded (kv_nearest)
+    const float inv = DT == DT_F32 ? __fdiv_rn(1.f, beta) : __builtin_amdgcn_rcpf(beta);
+    uint32_t w[2][W];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) kv_nearest<BITS, DT == DT_F32 ? 2 : 1>(x[i], beta, inv, w[i]);
     if (!mine || slot < 0 || slot >= (int64_t)a.c.pages * a.c.page_size) return;
     const uint32_t page = u32div((uint32_t)slot, a.c.page_div), off = (uint32_t)slot - page * a.c.page_size;
     const int64_t base = ((int64_t)page * a.c.heads + head) * a.c.page_size;
-    uint32_t* dst = (value ? a.c.v : a.c.k) + kv_word<BITS>(a.c, value, base, off, lane);
-    if constexpr (BITS == 4)
-        *dst = w[0];
-    else
-        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    uint32_t* dst = (value ? a.c.v : a.c.k) + kv_word<BITS>(a.c, value, base, off, 2 * lane);
+    if (value) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (W == 1)
+                dst[4 * i] = w[i][0];
+            else
+                *reinterpret_cast<uint2*>(dst + 8 * i) = make_uint2(w[i][0], w[i][1]);
+        }
+    } else if constexpr (W == 1) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0][0], w[1][0]);
+    } else {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
+    }
     if (lane == 0) reinterpret_cast<uint16_t*>(a.c.scales + base + off)[value ? 1 : 0] = (uint16_t)scale;
 }
 
+// A lane reads one block of each of kTokens tokens, whose slots, words and
+// scales are each loaded together.
+constexpr int kTokens = 4;
 template <int BITS, int DT, int GW>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvRowsArgs a)
 {
+    constexpr int W = BITS / 4, kGroups = kThreads / GW;
     const int lane = threadIdx.x % GW;
-    const int64_t t = (int64_t)blockIdx.x * (kThreads / GW) + threadIdx.x / GW;
+    const int64_t t0 = (int64_t)blockIdx.x * (kTokens * kGroups) + threadIdx.x / GW;
     const bool value = blockIdx.y & 1;
     const uint32_t head = blockIdx.y >> 1;
-    if (t >= a.n || lane >= (a.c.dim >> 3)) return;
-    const int64_t slot = a.slots[t];
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (slot >= 0 && slot < (int64_t)a.c.pages * a.c.page_size) {
-        const uint32_t page = u32div((uint32_t)slot, a.c.page_div), off = (uint32_t)slot - page * a.c.page_size;
+    if (lane >= (a.c.dim >> 3)) return;
+    int64_t slot[kTokens];
+#pragma unroll
+    for (int i = 0; i < kTokens; ++i) slot[i] = t0 + i * kGroups < a.n ? a.slots[t0 + i * kGroups] : -1;
+    uint32_t w[kTokens][W], both[kTokens];
+#pragma unroll
+    for (int i = 0; i < kTokens; ++i) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[i][j] = 0;
+        both[i] = 0;
+        if (slot[i] < 0 || slot[i] >= (int64_t)a.c.pages * a.c.page_size) continue;   // zeros
+        const uint32_t page = u32div((uint32_t)slot[i], a.c.page_div), off = (uint32_t)slot[i] - page * a.c.page_size;
         const int64_t base = ((int64_t)page * a.c.heads + head) * a.c.page_size;
         const uint32_t* src = (value ? a.c.v : a.c.k) + kv_word<BITS>(a.c, value, base, off, lane);
-        uint32_t w[BITS / 4];
-        if constexpr (BITS == 4) {
-            w[0] = *src;
+        if constexpr (W == 1) {
+            w[i][0] = *src;
         } else {
             const uint2 u = *reinterpret_cast<const uint2*>(src);
-            w[0] = u.x;
-            w[1] = u.y;
+            w[i][0] = u.x;
+            w[i][1] = u.y;
         }
-        const uint32_t both = a.c.scales[base + off];
-        const float beta = __uint_as_float(value ? both & 0xffff0000u : both << 16);
-        kv_point<BITS>(w, x);
+        both[i] = a.c.scales[base + off];
+    }
+#pragma unroll
+    for (int i = 0; i < kTokens; ++i) {
+        const int64_t t = t0 + i * kGroups;
+        if (t >= a.n) break;
+        const float beta = __uint_as_float(value ? both[i] & 0xffff0000u : both[i] << 16);
+        float x[8];
+        kv_point<BITS>(w[i], x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] *= beta;
+        store_n<DT, 8>(value ? a.v_out : a.k_out, (t * a.c.heads + head) * (int64_t)a.c.dim + 8 * lane, x);
     }
-    store_n<DT, 8>(value ? a.v_out : a.k_out, (t * a.c.heads + head) * (int64_t)a.c.dim + 8 * lane, x);
 }
 
 template <int BITS, int DT, int GW, bool WRITE>
 hipError_t launch(const KvRowsArgs& a, hipStream_t s)
 {
-    const dim3 grid((unsigned)((a.n + kThreads / GW - 1) / (kThreads / GW)), 2 * a.c.heads);
+    // GW: lanes of a vector, one or (write) two blocks each
+    const int64_t per = kThreads / GW * (WRITE ? 1 : kTokens);
+    const dim3 grid((unsigned)((a.n + per - 1) / per), 2 * a.c.heads);
     if constexpr (WRITE)
         hipLaunchKernelGGL((kv_write_kernel<BITS, DT, GW>), grid, dim3(kThreads), 0, s, a);
     else
@@ -117,10 +165,10 @@ template <int BITS, int DT, bool WRITE>
 hipError_t by_width(const KvRowsArgs& a, hipStream_t s)
 {
     const int nb = a.c.dim / 8;
-    if (nb <= 4) return launch<BITS, DT, 4, WRITE>(a, s);
-    if (nb <= 8) return launch<BITS, DT, 8, WRITE>(a, s);
-    if (nb <= 16) return launch<BITS, DT, 16, WRITE>(a, s);
-    return launch<BITS, DT, 32, WRITE>(a, s);
+    if (nb <= 4) return launch<BITS, DT, WRITE ? 2 : 4, WRITE>(a, s);
+    if (nb <= 8) return launch<BITS, DT, WRITE ? 4 : 8, WRITE>(a, s);
+    if (nb <= 16) return launch<BITS, DT, WRITE ? 8 : 16, WRITE>(a, s);
+    return launch<BITS, DT, WRITE ? 16 : 32, WRITE>(a, s);
 }
 
 template <bool WRITE>

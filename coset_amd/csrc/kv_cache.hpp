@@ -83,49 +83,102 @@ __device__ __forceinline__ uint32_t kv_scale_bits(float amax)
 // and a move at distance e adds beta^2 - 2 beta e, so the choice needs the
 // sum, the largest and the smallest |r| only.  Equal distances go to the
 // integers, equal remainders to the first coordinate.
-template <int BITS>
+//
+// round() is an addition of 1.5 * 2^23 + 2^(BITS-1), which leaves the field in
+// the low byte.  STEPS: of the quotient (div_by_recip).  Two give fp32's
+// correctly rounded quotient for any x.  One gives it where it is
+// representable, exact halves among them, and else one to an ulp: enough for
+// x of 11 bits, whose quotients by 8-bit scales lie 2^-12 or more (relatively)
+// from a half that they do not hit.
+// The fields are packed first; moves and the halves' subtractions are then
+// additions to the packed word, which cannot carry: every field stays within
+// its bits before and after.
+__device__ __forceinline__ float kv_largest(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float kv_smallest(float a, float b, float c)
+{
+    float r;
+    asm("v_min3_f32 %0, |%1|, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+template <int BITS, int STEPS>
 __device__ __forceinline__ void kv_nearest(const float (&x)[8], float beta, float inv, uint32_t (&w)[BITS / 4])
 {
-    float r[8], a[8];
-    int c[8];
-    int sum = 0, neg = 0;
+    constexpr float kRound = 12582912.f + (float)(1 << (BITS - 1));
+    float r[8];
+    uint32_t c[8], signs = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float f = rintf(div_by_recip<2>(x[j], beta, inv));
-        r[j] = fmaf(-f, beta, x[j]);
-        a[j] = fabsf(r[j]);
-        c[j] = (int)f;
-        sum ^= c[j];
-        neg ^= r[j] < 0.f ? 1 : 0;
+    for (int j = 7; j >= 0; --j) {
+        const float t = __fadd_rn(div_by_recip<STEPS>(x[j], beta, inv), kRound);
+        r[j] = fmaf(-__fsub_rn(t, kRound), beta, x[j]);   // never -0
+        c[j] = __float_as_uint(t);
+        signs = __builtin_amdgcn_alignbit(signs, __float_as_uint(r[j]), 31);   // bit j: r_j < 0
     }
-    const float s = __fadd_rn(__fadd_rn(__fadd_rn(a[0], a[4]), __fadd_rn(a[2], a[6])),
-                              __fadd_rn(__fadd_rn(a[1], a[5]), __fadd_rn(a[3], a[7])));
-    const float most = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(a[4], a[5]), fmaxf(a[6], a[7])));
-    const float least = fminf(fminf(fminf(a[0], a[1]), fminf(a[2], a[3])), fminf(fminf(a[4], a[5]), fminf(a[6], a[7])));
-    const bool odd_f = sum & 1, odd_g = (sum ^ neg) & 1;
+    const float s = __fadd_rn(__fadd_rn(__fadd_rn(fabsf(r[0]), fabsf(r[4])), __fadd_rn(fabsf(r[2]), fabsf(r[6]))),
+                              __fadd_rn(__fadd_rn(fabsf(r[1]), fabsf(r[5])), __fadd_rn(fabsf(r[3]), fabsf(r[7]))));
+    const float most = kv_largest(kv_largest(r[0], r[1], r[2]), kv_largest(r[3], r[4], r[5]), kv_largest(r[6], r[7], r[7]));
+    const float least = kv_smallest(kv_smallest(r[0], r[1], r[2]), kv_smallest(r[3], r[4], r[5]), kv_smallest(r[6], r[7], r[7]));
+    // fields and sign bits in their places, and the parity of the fields' sum
+    uint32_t down[BITS / 4];
+    uint32_t low;
+    if constexpr (BITS == 4) {
+        const uint32_t p0 = (c[1] << 4) | c[0], p1 = (c[3] << 4) | c[2], p2 = (c[5] << 4) | c[4], p3 = (c[7] << 4) | c[6];
+        const uint32_t lo = __builtin_amdgcn_perm(p1, p0, 0x0c0c0400u), hi = __builtin_amdgcn_perm(p3, p2, 0x0c0c0400u);
+        w[0] = (hi << 16) | lo;
+        low = w[0] & 0x11111111u;
+        uint32_t d = (signs | signs << 12) & 0x000f000fu;
+        d = (d | d << 6) & 0x03030303u;
+        down[0] = (d | d << 3) & 0x11111111u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t lo = __builtin_amdgcn_perm(c[4 * i + 1], c[4 * i], 0x0c0c0400u);
+            const uint32_t hi = __builtin_amdgcn_perm(c[4 * i + 3], c[4 * i + 2], 0x0c0c0400u);
+            w[i] = (hi << 16) | lo;
+            uint32_t d = (signs >> (4 * i)) & 15u;
+            d = (d | d << 14) & 0x00030003u;
+            down[i] = (d | d << 7) & 0x01010101u;
+        }
+        low = (w[0] ^ w[1]) & 0x01010101u;
+    }
+    const uint32_t odd = __popc(low);
+    const bool odd_f = odd & 1, odd_g = (odd + __popc(signs)) & 1;
     const float lhs = __fadd_rn(__fsub_rn(2.f * beta, s), odd_g ? 2.f * least : 0.f);
     const float rhs = odd_f ? __fsub_rn(beta, 2.f * most) : 0.f;
     const bool half = lhs < rhs;
     const float target = half ? least : most;
-    bool move = half ? odd_g : odd_f;
-    constexpr int kBias = 1 << (BITS - 1);
+    // the first coordinate at the target: its field's unit and its remainder
+    float at = r[7];
+    uint32_t unit = 1u << 28;
+    if constexpr (BITS == 8) unit = 56;   // its field's shift in the two words
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const bool down = r[j] < 0.f;
-        c[j] += kBias - ((half && down) ? 1 : 0);
-        const bool hit = move && a[j] == target;
-        c[j] += hit ? (down == half ? 1 : -1) : 0;
-        move = move && !hit;
+    for (int j = 6; j >= 0; --j) {
+        const bool hit = fabsf(r[j]) == target;
+        at = hit ? r[j] : at;
+        unit = hit ? (BITS == 4 ? 1u << (4 * j) : 8u * j) : unit;
     }
-    c[7] = (c[7] & ~1) | (half ? 1 : 0);
-    constexpr int kPer = 32 / BITS;
+    const bool move = half ? odd_g : odd_f;
+    const bool up = (at < 0.f) == half;
+    uint32_t step[BITS / 4];
+    if constexpr (BITS == 4) {
+        step[0] = move ? unit : 0u;
+    } else {
+        const uint32_t one = move ? 1u << (unit & 31) : 0u;
+        step[0] = unit < 32 ? one : 0u;
+        step[1] = unit < 32 ? 0u : one;
+    }
 #pragma unroll
     for (int i = 0; i < BITS / 4; ++i) {
-        uint32_t u = 0;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) u |= (uint32_t)c[i * kPer + j] << (BITS * j);
-        w[i] = u;
+        w[i] -= half ? down[i] : 0u;
+        w[i] += up ? step[i] : 0u - step[i];
     }
+    constexpr uint32_t kH = 1u << (32 - BITS);
+    w[BITS / 4 - 1] = (w[BITS / 4 - 1] & ~kH) | (half ? kH : 0u);
 }
 
 // A block's coordinates.
