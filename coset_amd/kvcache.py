@@ -90,14 +90,21 @@ def _dtype(dt: torch.dtype) -> int:
     return code
 
 
-def _on_device(cache: E8KVCache, **tensors) -> torch.device:
+def _device(cache: E8KVCache) -> torch.device:
     dev = cache.k.device
     if dev.type != "cuda":
         raise _lib.CosetError("the cache is not on a GPU")
-    for name, t in tensors.items():
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
     return dev
+
+
+def _same(dev: torch.device, name: str, t: torch.Tensor) -> None:
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+
+
+def is_current(dev: torch.device) -> bool:
+    """Whether kernels that are launched now run on dev (the calls below switch to it where they do not)."""
+    return torch._C._cuda_getDevice() == dev.index
 
 
 def _slots(slots: torch.Tensor, n: Optional[int]) -> torch.Tensor:
@@ -127,13 +134,18 @@ def kv_write(cache: E8KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Te
     if k.dtype != v.dtype:
         raise ValueError(f"k is {k.dtype}, v {v.dtype}")
     dt = _dtype(k.dtype)
-    dev = _on_device(cache, k=k, v=v, slots=slots)
+    dev = _device(cache)
+    _same(dev, "k", k)
+    _same(dev, "v", v)
+    _same(dev, "slots", slots)
+    if not is_current(dev):
+        with torch.cuda.device(dev):
+            return kv_write(cache, k, v, slots)
     n = k.shape[0]
     slots = _slots(slots, n)
     k, v = _rows(k), _rows(v)
-    with torch.cuda.device(dev):
-        _lib.call("coset_kv_write", cache._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                  v.stride(1), dt, slots.data_ptr(), n, _lib.stream_of(k))
+    _lib.call("coset_kv_write", cache._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+              v.stride(1), dt, slots.data_ptr(), n, _lib.stream_of(k))
 
 
 def kv_read(cache: E8KVCache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16
@@ -142,14 +154,16 @@ def kv_read(cache: E8KVCache, slots: torch.Tensor, dtype: torch.dtype = torch.bf
     in ``dtype`` (beta lambda in fp32, rounded once).  Rows outside the cache
     are zeros."""
     dt = _dtype(dtype)
-    dev = _on_device(cache, slots=slots)
+    dev = _device(cache)
+    _same(dev, "slots", slots)
+    if not is_current(dev):
+        with torch.cuda.device(dev):
+            return kv_read(cache, slots, dtype)
     slots = _slots(slots, None)
     n = slots.shape[0]
-    with torch.cuda.device(dev):
-        k = torch.empty((n, cache.kv_heads, cache.head_dim), dtype=dtype, device=dev)
-        v = torch.empty_like(k)
-        _lib.call("coset_kv_read", cache._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), dt,
-                  _lib.stream_of(k))
+    k = torch.empty((n, cache.kv_heads, cache.head_dim), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    _lib.call("coset_kv_read", cache._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), dt, _lib.stream_of(k))
     return k, v
 
 
@@ -208,32 +222,36 @@ def kv_attention(q: torch.Tensor, cache: E8KVCache, block_table: torch.Tensor, l
     seqs, max_pages = block_table.shape
     if lengths.shape != (seqs,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
         raise ValueError(f"lengths must be a contiguous int32 vector of {seqs}")
-    dev = _on_device(cache, q=q, block_table=block_table, lengths=lengths)
+    dev = _device(cache)
+    _same(dev, "q", q)
+    _same(dev, "block_table", block_table)
+    _same(dev, "lengths", lengths)
     if cu_queries is not None:
         if cu_queries.shape != (seqs + 1,) or cu_queries.dtype != torch.int32 or not cu_queries.is_contiguous():
             raise ValueError(f"cu_queries must be a contiguous int32 vector of {seqs + 1}")
-        if cu_queries.device != dev:
-            raise ValueError(f"cu_queries is on {cu_queries.device}, the cache on {dev}")
+        _same(dev, "cu_queries", cu_queries)
     words = 0
     if tree_mask is not None:
         if tree_mask.dim() != 2 or tree_mask.shape[0] != n or tree_mask.shape[1] < 1 or \
                 tree_mask.dtype != torch.int64 or not tree_mask.is_contiguous():
             raise ValueError(f"tree_mask must be contiguous int64 [{n}, words]")
-        if tree_mask.device != dev:
-            raise ValueError(f"tree_mask is on {tree_mask.device}, the cache on {dev}")
+        _same(dev, "tree_mask", tree_mask)
         words = tree_mask.shape[1]
+    if not is_current(dev):
+        with torch.cuda.device(dev):
+            return kv_attention(q, cache, block_table, lengths, cu_queries=cu_queries, tree_mask=tree_mask,
+                                scale=scale, return_lse=return_lse, workspace=workspace)
     q = _rows(q)
-    with torch.cuda.device(dev):
-        out = torch.empty((n, heads, dim), dtype=q.dtype, device=dev)
-        lse = torch.empty((n, heads), dtype=torch.float32, device=dev) if return_lse else None
-        need = _lib.load().coset_kv_attention_workspace_floats(cache._ref, n, seqs, heads, dt, max_pages)
-        if workspace is None or workspace.numel() < need:
-            workspace = torch.empty(need, dtype=torch.float32, device=dev)
-        elif workspace.device != dev or workspace.dtype != torch.float32 or not workspace.is_contiguous():
-            raise ValueError("workspace must be contiguous fp32 on the cache's device")
-        _lib.call("coset_kv_attention", cache._ref, q.data_ptr(), q.stride(0), q.stride(1), dt, n, heads, seqs,
-                  None if cu_queries is None else cu_queries.data_ptr(), lengths.data_ptr(), block_table.data_ptr(),
-                  block_table.stride(0), max_pages, None if tree_mask is None else tree_mask.data_ptr(), words,
-                  dim ** -0.5 if scale is None else float(scale), out.data_ptr(), _lib.ptr(lse),
-                  workspace.data_ptr(), workspace.numel(), _lib.stream_of(q))
+    out = torch.empty((n, heads, dim), dtype=q.dtype, device=dev)
+    lse = torch.empty((n, heads), dtype=torch.float32, device=dev) if return_lse else None
+    need = _lib.load().coset_kv_attention_workspace_floats(cache._ref, n, seqs, heads, dt, max_pages)
+    if workspace is None or workspace.numel() < need:
+        workspace = torch.empty(need, dtype=torch.float32, device=dev)
+    elif workspace.device != dev or workspace.dtype != torch.float32 or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous fp32 on the cache's device")
+    _lib.call("coset_kv_attention", cache._ref, q.data_ptr(), q.stride(0), q.stride(1), dt, n, heads, seqs,
+              None if cu_queries is None else cu_queries.data_ptr(), lengths.data_ptr(), block_table.data_ptr(),
+              block_table.stride(0), max_pages, None if tree_mask is None else tree_mask.data_ptr(), words,
+              dim ** -0.5 if scale is None else float(scale), out.data_ptr(), None if lse is None else lse.data_ptr(),
+              workspace.data_ptr(), workspace.numel(), _lib.stream_of(q))
     return (out, lse) if return_lse else out

@@ -5,13 +5,13 @@ has no attention.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from .kvcache import _dtype, _rows
+from .kvcache import _dtype, _rows, is_current
 
 
 def rope_table(length: int, rot: int, base: float = 10000.0, device: Optional[torch.device] = None) -> torch.Tensor:
@@ -25,30 +25,32 @@ def rope_table(length: int, rot: int, base: float = 10000.0, device: Optional[to
     return torch.cat([angle.cos(), angle.sin()], dim=1).float()
 
 
+# coset_rope_side and coset_rope, packed in one call each (a ctypes structure takes several times as long)
+_SIDE = struct.Struct("=5Q5q")
+_PLAN = struct.Struct("=2Q3q11if")
+
+
 def _side(x, out, weight, grad=None, weight_grad=None):
-    return _lib.RopeSideStruct(
-        x.data_ptr(), None if grad is None else grad.data_ptr(), out.data_ptr(),
-        None if weight is None else weight.data_ptr(), None if weight_grad is None else weight_grad.data_ptr(),
-        x.stride(0), x.stride(1), 0 if grad is None else grad.stride(0), 0 if grad is None else grad.stride(1),
-        x.shape[1])
+    gt, gh = (0, 0) if grad is None else (grad.stride(0), grad.stride(1))
+    return _SIDE.pack(x.data_ptr(), 0 if grad is None else grad.data_ptr(), out.data_ptr(),
+                      0 if weight is None else weight.data_ptr(), 0 if weight_grad is None else weight_grad.data_ptr(),
+                      x.stride(0), x.stride(1), gt, gh, x.shape[1])
 
 
 def _plan(q, table, positions, wq, wk, eps, bounds, interleaved, norm):
     w = wq if wq is not None else wk
-    return _lib.RopeStruct(
-        table.data_ptr(), positions.data_ptr(), q.shape[0], table.shape[0], positions.stride(0), q.shape[2],
-        table.shape[1], positions.shape[0], bounds, norm, interleaved, _dtype(q.dtype),
-        _lib.F32 if w is None else _dtype(w.dtype), eps)
+    n, _, dim = q.shape
+    length, rot = table.shape
+    return _PLAN.pack(table.data_ptr(), positions.data_ptr(), n, length, positions.stride(0), dim, rot,
+                      positions.shape[0], *bounds, norm, interleaved, _dtype(q.dtype),
+                      _lib.F32 if w is None else _dtype(w.dtype), eps)
 
 
 def _forward(q, k, table, positions, wq, wk, eps, bounds, interleaved, norm):
-    with torch.cuda.device(q.device):
-        oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        r = _plan(q, table, positions, wq, wk, eps, bounds, interleaved, norm)
-        sq, sk = _side(q, oq, wq), _side(k, ok, wk)
-        _lib.call("coset_qk_norm_rope_fwd", ctypes.addressof(r), ctypes.addressof(sq), ctypes.addressof(sk),
-                  _lib.stream_of(q))
+    oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _lib.call("coset_qk_norm_rope_fwd", _plan(q, table, positions, wq, wk, eps, bounds, interleaved, norm),
+              _side(q, oq, wq), _side(k, ok, wk), _lib.stream_of(q))
     return oq, ok
 
 
@@ -63,38 +65,33 @@ class _NormRope(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         q, k, wq, wk, table, positions = ctx.saved_tensors
-        eps, bounds, interleaved, norm = ctx.rest
-        gq, gk = _rows(gq), _rows(gk)
-        with torch.cuda.device(q.device):
-            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
-            dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
-            need = 0
-            ws = None
-            if dwq is not None or dwk is not None:
-                need = _lib.load().coset_qk_norm_rope_workspace_floats(q.shape[0], q.shape[2])
-                ws = torch.empty(need, dtype=torch.float32, device=q.device)
-            r = _plan(q, table, positions, wq, wk, eps, bounds, interleaved, norm)
-            sq, sk = _side(q, dq, wq, gq, dwq), _side(k, dk, wk, gk, dwk)
-            _lib.call("coset_qk_norm_rope_bwd", ctypes.addressof(r), ctypes.addressof(sq), ctypes.addressof(sk),
-                      _lib.ptr(ws), need, _lib.stream_of(q))
+        if not is_current(q.device):
+            with torch.cuda.device(q.device):
+                return _NormRope._gradients(ctx, q, k, wq, wk, table, positions, _rows(gq), _rows(gk))
+        return _NormRope._gradients(ctx, q, k, wq, wk, table, positions, _rows(gq), _rows(gk))
+
+    @staticmethod
+    def _gradients(ctx, q, k, wq, wk, table, positions, gq, gk):
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
+        dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
+        need, ws = 0, None
+        if dwq is not None or dwk is not None:
+            need = _lib.load().coset_qk_norm_rope_workspace_floats(q.shape[0], q.shape[2])
+            ws = torch.empty(need, dtype=torch.float32, device=q.device)
+        _lib.call("coset_qk_norm_rope_bwd", _plan(q, table, positions, wq, wk, *ctx.rest), _side(q, dq, wq, gq, dwq),
+                  _side(k, dk, wk, gk, dwk), None if ws is None else ws.data_ptr(), need, _lib.stream_of(q))
         return dq, dk, dwq, dwk, None, None, None, None, None, None
 
 
-_BOUNDS = {}
-
-
-def _bounds(sections: Tuple[int, ...]):
-    """ctypes int32[4]: the first pair behind each axis's section."""
-    b = _BOUNDS.get(sections)
-    if b is None:
-        at, ends = 0, []
-        for s in sections:
-            at += s
-            ends.append(at)
-        b = _BOUNDS[sections] = (ctypes.c_int32 * 4)(*ends)
-    return b
+def _bounds(sections: Tuple[int, ...]) -> Tuple[int, ...]:
+    """The first pair behind each axis's section, for four axes."""
+    at, ends = 0, []
+    for n in sections:
+        at += n
+        ends.append(at)
+    return tuple(ends + [at] * (4 - len(ends)))
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, positions: torch.Tensor,
@@ -159,6 +156,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, position
         norm = weighted
     elif not norm and weighted:
         raise ValueError("weights without the norm")
+    if not is_current(dev):
+        with torch.cuda.device(dev):
+            return qk_norm_rope(q, k, table, positions, q_weight, k_weight, eps=eps, sections=sections,
+                                interleaved=interleaved, norm=norm)
     if positions.stride(1) != 1:
         positions = positions.contiguous()
     q, k = _rows(q), _rows(k)
