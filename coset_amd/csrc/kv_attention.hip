@@ -80,10 +80,17 @@ struct Desc {
     int pad[3];
 };
 
+// A sequence's part of the line: its key heads one after another, and of
+// each the row tiles in pairs, the last with the first and so on inwards.  A
+// tile's steps end at the last token that any of its rows sees, which for the
+// new tokens of a prompt grows evenly with the tile, so that all pairs take the
+// same number of steps (to the rounding, which leaves the smaller tile a step or
+// two without tokens) and a place on the line is found by division.
 struct Work {
-    int steps;       // in a segment
     int tiles;       // row tiles
-    int units;       // steps * tiles * key heads
+    int pair;        // steps of two paired tiles
+    int head;        // steps of a key head
+    int units;       // of all key heads
 };
 
 struct Seq {
@@ -106,13 +113,36 @@ __device__ __forceinline__ Seq seq_of(const KvAttentionArgs& a, int b)
     return s;
 }
 
+// Tokens that any row of the tile may see.
+__device__ __forceinline__ int reach_of(const KvAttentionArgs& a, const Seq& s, int rows, int tile)
+{
+    if (a.mask) return s.length;
+    const int last = min((tile + 1) * rows, s.tokens * a.group) - 1;
+    return min(s.length, s.length - s.tokens + (int)u32div((uint32_t)last, a.group_div) + 1);
+}
+
 // span: tokens of a step
+__device__ __forceinline__ int steps_of(const KvAttentionArgs& a, const Seq& s, int rows, int span, int tile)
+{
+    return max((reach_of(a, s, rows, tile) + span - 1) / span, 1);
+}
+
 __device__ __forceinline__ Work work_of(const KvAttentionArgs& a, const Seq& s, int rows, int span)
 {
-    Work w;
-    w.steps = max((s.length + span - 1) / span, 1);
+    Work w{};
     w.tiles = (s.tokens * a.group + rows - 1) / rows;
-    w.units = w.steps * w.tiles * (int)a.c.heads;
+    if (w.tiles < 2) {
+        w.head = w.tiles ? steps_of(a, s, rows, span, 0) : 0;
+        w.units = w.head * (int)a.c.heads;
+        return w;
+    }
+    const int ctx = s.length - s.tokens;
+    const int64_t full = 2 * (int64_t)max((s.length + span - 1) / span, 1);
+    // sum of two paired tiles' reaches, each rounded up
+    const int64_t both = 2 * (int64_t)ctx + 2 + (int64_t)u32div((uint32_t)(w.tiles + 1) * (uint32_t)rows - 2u, a.group_div);
+    w.pair = (int)(a.mask || ctx < 0 ? full : min(full, (both + 2 * (span - 1)) / span));
+    w.head = w.tiles / 2 * w.pair + (w.tiles & 1 ? steps_of(a, s, rows, span, w.tiles / 2) : 0);
+    w.units = w.head * (int)a.c.heads;
     return w;
 }
 
@@ -631,9 +661,23 @@ __device__ __forceinline__ int over_lanes(int u, int lane)
 // A workgroup's run of the line of units.
 struct Line {
     int unit, end, run;
-    int b, seg, step;   // where it begins: sequence, its segment, the segment's step
+    int b, kh, at;      // where it is: sequence, its key head, the step on that head's part of the line
+    int tile, steps, step;   // the row tile there, its steps, and which of them
     Seq sq;
     Work wk;
+
+    __device__ __forceinline__ void place(const KvAttentionArgs& a, int rows, int span)
+    {
+        const int pairs = wk.tiles / 2, pair = pairs ? min(at / wk.pair, pairs) : 0;
+        step = at - pair * wk.pair;
+        tile = wk.tiles - 1 - pair;
+        steps = steps_of(a, sq, rows, span, tile);
+        if (pair < pairs && step >= steps) {
+            step -= steps;
+            steps = wk.pair - steps;
+            tile = pair;
+        }
+    }
 
     // false: nothing to do
     __device__ __forceinline__ bool begin(const KvAttentionArgs& a, int id, int blocks, int rows, int span, int lane)
@@ -649,7 +693,7 @@ struct Line {
         unit = id * run;
         end = min(unit + run, total);
         if (unit >= end) return false;
-        int at = 0, before = 0;
+        int found = 0, before = 0;
         for (int b0 = 0; b0 < a.seqs; b0 += 64) {
             if (a.seqs > 64) {
                 u = b0 + lane < a.seqs ? work_of(a, seq_of(a, b0 + lane), rows, span).units : 0;
@@ -658,36 +702,42 @@ struct Line {
             const uint64_t past = __ballot(before + sum > unit);
             if (past) {
                 const int first = __ffsll((unsigned long long)past) - 1;
-                at = b0 + first;
+                found = b0 + first;
                 before += __builtin_amdgcn_readlane(sum - u, first);
                 break;
             }
             before += __builtin_amdgcn_readlane(sum, 63);
         }
-        b = __builtin_amdgcn_readfirstlane(at);
+        b = __builtin_amdgcn_readfirstlane(found);
         before = __builtin_amdgcn_readfirstlane(before);
         sq = seq_of(a, b);
         wk = work_of(a, sq, rows, span);
-        seg = (unit - before) / wk.steps;
-        step = (unit - before) % wk.steps;
         // past the sequence: starts that overlap so far that the line's length wrapped
-        return seg < wk.tiles * (int)a.c.heads;
+        if (unit - before < 0 || unit - before >= wk.units) return false;
+        kh = (unit - before) / wk.head;
+        at = (unit - before) % wk.head;
+        place(a, rows, span);
+        return true;
     }
 
     // behind `count` steps of the segment; false at the run's end
     __device__ __forceinline__ bool next(const KvAttentionArgs& a, int count, int rows, int span)
     {
         unit += count;
-        step = 0;
         if (unit >= end) return false;
-        if (++seg == wk.tiles * (int)a.c.heads) {
-            seg = 0;
-            do {
-                if (++b >= a.seqs) return false;
-                sq = seq_of(a, b);
-                wk = work_of(a, sq, rows, span);
-            } while (wk.units == 0);
+        at += count;
+        if (at == wk.head) {
+            at = 0;
+            if (++kh == (int)a.c.heads) {
+                kh = 0;
+                do {
+                    if (++b >= a.seqs) return false;
+                    sq = seq_of(a, b);
+                    wk = work_of(a, sq, rows, span);
+                } while (wk.units == 0);
+            }
         }
+        place(a, rows, span);
         return true;
     }
 };
@@ -710,7 +760,7 @@ struct Parts {
 __device__ __forceinline__ void leave(const Parts& parts, const KvAttentionArgs& a, const Line& ln, int id, int kh, int row0, int rows, int count)
 {
     Desc d{};
-    d.parts = min(1 + (ln.wk.steps - count + ln.run - 1) / ln.run, (int)gridDim.x - id);
+    d.parts = min(1 + (ln.steps - count + ln.run - 1) / ln.run, (int)gridDim.x - id);
     d.row0 = row0;
     d.rows = rows;
     d.token0 = ln.sq.token0;
@@ -779,12 +829,12 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
     int count;
     do {
         const Seq& sq = ln.sq;
-        count = min(ln.wk.steps - ln.step, ln.end - ln.unit);
-        const int kh = ln.seg / ln.wk.tiles, tile = ln.seg % ln.wk.tiles;
+        count = min(ln.steps - ln.step, ln.end - ln.unit);
+        const int kh = ln.kh, tile = ln.tile;
         const int row0 = tile * kRows, rows = min(sq.tokens * a.group - row0, kRows);
         const int ctx = sq.length - sq.tokens;
         // tokens that any row of the tile may see, and those that all see
-        const int reach = a.mask ? sq.length : min(sq.length, ctx + (int)u32div((uint32_t)(row0 + rows - 1), a.group_div) + 1);
+        const int reach = reach_of(a, sq, kRows, tile);
         const int all = a.mask ? ctx : ctx + (int)u32div((uint32_t)row0, a.group_div) + 1;
         const Pages pages(a, ln.b, kh);
         int token = (ln.step * kWaves + wave) * kTile;
@@ -860,7 +910,7 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
 
         // the four waves' rows
         const int tid = here(threadIdx.x), g = (tid & 63) >> 4, n = tid & 15;
-        const bool done = count == ln.wk.steps;
+        const bool done = count == ln.steps;
         const int64_t slot = 2 * id + (ln.step == 0 ? 1 : 0);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
@@ -976,13 +1026,13 @@ __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArg
     int count;
     do {
         const Seq& sq = ln.sq;
-        count = min(ln.wk.steps - ln.step, ln.end - ln.unit);
-        const int kh = ln.seg / ln.wk.tiles, tile = ln.seg % ln.wk.tiles;
+        count = min(ln.steps - ln.step, ln.end - ln.unit);
+        const int kh = ln.kh, tile = ln.tile;
         const int row0 = tile * kRows, rows = min(sq.tokens * a.group - row0, kRows);
         const int ctx = sq.length - sq.tokens;
         // the wave's own rows
         const int first = row0 + wave * 16 * NR, last = min(first + 16 * NR, row0 + rows) - 1;
-        const int reach = a.mask ? sq.length : min(sq.length, ctx + (int)u32div((uint32_t)(row0 + rows - 1), a.group_div) + 1);
+        const int reach = reach_of(a, sq, kRows, tile);
         const int mine = last < first ? 0 : a.mask ? sq.length : min(sq.length, ctx + (int)u32div((uint32_t)last, a.group_div) + 1);
         const int all = a.mask ? ctx : ctx + (int)u32div((uint32_t)first, a.group_div) + 1;
         const Pages pages(a, ln.b, kh);
@@ -1119,7 +1169,7 @@ __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArg
             __syncthreads();
         }
 
-        const bool done = count == ln.wk.steps;
+        const bool done = count == ln.steps;
         const int tid = here(threadIdx.x), g = (tid & 63) >> 4, n = tid & 15;
         const int64_t slot = 2 * id + (ln.step == 0 ? 1 : 0);
 #pragma unroll

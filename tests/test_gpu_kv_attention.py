@@ -95,6 +95,20 @@ def test_chunks(heads, kv, counts, dtype, dim, bits):
     _run(ca, cache, lengths, counts, heads, dtype, _table(3, most, cache.pages, 2))
 
 
+@pytest.mark.parametrize("dtype,dim,bits", [(torch.bfloat16, 128, 4), (torch.float16, 256, 4), (torch.float32, 64, 8)])
+@pytest.mark.parametrize("heads,kv", [(2, 2), (8, 1), (6, 2)])
+def test_whole_prompts(heads, kv, dtype, dim, bits):
+    """Prompts from their first token on, whose rows see from one token to all of them: many row tiles of a sequence,
+    odd and even numbers of them, beside one behind a context and one with more new tokens than cached ones."""
+    import coset_amd as ca
+    print(f"whole prompts dim={dim} bits={bits} heads={heads}/{kv} {dtype}", flush=True)
+    page = 32
+    for counts, lengths in (([400, 129, 1, 257], [400, 129, 5, 300]), ([65], [65]), ([330], [400]), ([300, 40], [200, 40])):
+        most = -(-max(lengths) // page)
+        cache = _fill(ca, len(counts) * most, page, kv, dim, bits, 13)
+        _run(ca, cache, lengths, counts, heads, dtype, _table(len(counts), most, cache.pages, 4))
+
+
 @pytest.mark.parametrize("dtype,dim,bits", [(torch.bfloat16, 128, 8), (torch.float16, 128, 4), (torch.float32, 64, 4)])
 def test_trees(dtype, dim, bits):
     """Trees of drafted tokens over a context, some with no context, some rows that see nothing, and two mask words."""
