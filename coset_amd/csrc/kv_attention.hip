@@ -794,7 +794,10 @@ __device__ __forceinline__ int xcd_id()
 }
 
 // Up to 32 rows: every wave holds all of them and takes 32 tokens of each
-// step, decoding words straight into operands.
+// step, decoding words straight into operands.  64 sequences of 1000 to 8192
+// tokens, 32 / 8 heads of 128, 4 bits: 74 us with the join, 4.2 TB/s of the
+// cache's bytes; the vector units are busy 75 % of the cycles (decode: about 3
+// instructions for 8 values of each side, and the weights), the matrix cores 18 %.
 // DP: dim padded to 64, 128 or 256; NR: 16-row tiles; QS: queries in two fp16
 // parts; PS: weights in two; OCC: waves a SIMD.
 template <int DP, int BITS, int NR, int DT, bool QS, bool PS, int OCC>
@@ -983,7 +986,11 @@ __global__ void __launch_bounds__(kThreads, OCC) kv_few_kernel(KvAttentionArgs a
 
 // More rows: WAVES waves hold 16 * NR rows each and share the tokens, which
 // they decode once into operands in LDS, an equal part each: one buffer is
-// filled while the other one is used.
+// filled while the other one is used.  A prompt of 16384 tokens, 32 / 8 heads of
+// 128, 4 bits: 2.93 ms, 750 TFLOP/s; trees of up to 32 tokens on 16 sequences to
+// 6000, 8 bits: 74 us.  Within a wave the vector work (decode, weights) and the
+// matrix cores' alternate, two waves a SIMD overlap them: vector units 46 %,
+// matrix cores 18 % of the trees' cycles.
 template <int DP, int BITS, int NR, int WAVES, int DT, bool QS, bool PS, int OCC>
 __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArgs a, int most_parts)
 {
@@ -1208,24 +1215,56 @@ __global__ void __launch_bounds__(64 * WAVES, OCC) kv_many_kernel(KvAttentionArg
     } while (ln.next(a, count, kRows, kSpan));
 }
 
-// Joins the parts of the segment that begins in workgroup blockIdx.x: one
-// workgroup a row (blockIdx.y), DP / 4 threads across the row, the rest of
-// them across the parts.
-template <int DP, int ROWS, int DT>
+// The first kernel's workgroup that the segment number `rank` of those left in
+// parts begins in; -1: there are fewer.
+__device__ __forceinline__ int begin_of(const Desc* descs, int blocks, int rank)
+{
+    __shared__ int sh_count[kWaves], sh_at;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int before = 0;
+    for (int base = 0; base < blocks; base += kThreads) {
+        const int i = base + (int)threadIdx.x;
+        const bool one = i < blocks && descs[i].parts != 0;
+        const uint64_t all = __ballot(one);
+        if (lane == 0) sh_count[wave] = __popcll(all);
+        if (threadIdx.x == 0) sh_at = -1;
+        __syncthreads();
+        int mine = before + __popcll(all & ((1ull << lane) - 1));
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            mine += w < wave ? sh_count[w] : 0;
+            before += sh_count[w];
+        }
+        if (one && mine == rank) sh_at = i;
+        __syncthreads();
+        const int at = sh_at;
+        if (at >= 0) return at;
+        __syncthreads();
+    }
+    return -1;
+}
+
+// Joins the parts of the segment that begins in workgroup blockIdx.x (FIND: of
+// the segment number blockIdx.x): one workgroup a row (blockIdx.y), DP / 4
+// threads across the row, the rest of them across the parts.
+template <int DP, int ROWS, int DT, bool FIND>
 __global__ void __launch_bounds__(kThreads) kv_join_kernel(KvAttentionArgs a, int blocks)
 {
     constexpr int kRows = ROWS;
     constexpr int kAcross = DP / 4, kParts = kThreads / kAcross;
     __shared__ __align__(16) float sh_o[kParts][DP];
     __shared__ float sh_m[kParts], sh_l[kParts];
-    const Desc d = reinterpret_cast<const Desc*>(a.workspace)[blockIdx.x];
+    const Desc* descs = reinterpret_cast<const Desc*>(a.workspace);
+    const int begin = FIND ? begin_of(descs, blocks, (int)blockIdx.x) : (int)blockIdx.x;
+    if (begin < 0) return;
+    const Desc d = descs[begin];
     const int row = blockIdx.y;
     if (d.parts == 0 || row >= d.rows) return;
     const Parts parts(a.workspace, blocks, kRows);
     const float* part_ml = parts.ml;
     const float* part_o = parts.o;
     const int across = threadIdx.x % kAcross, lot = threadIdx.x / kAcross;
-    auto slot = [&](int p) { return (int64_t)(2 * ((int)blockIdx.x + p) + (p == 0 ? 1 : 0)) * kRows + row; };
+    auto slot = [&](int p) { return (int64_t)(2 * (begin + p) + (p == 0 ? 1 : 0)) * kRows + row; };
     float m = kNone;
     for (int p = lot; p < d.parts; p += kParts) m = fmaxf(m, part_ml[slot(p) * 2]);
     if (across == 0) sh_m[lot] = m;
@@ -1290,6 +1329,13 @@ __global__ void __launch_bounds__(kThreads) kv_join_rows_kernel(KvAttentionArgs 
     if (a.lse && across == 0) a.lse[at] = some ? (m + log2f(l)) * (1.f / kLog2e) : -INFINITY;
 }
 
+// Parts a segment from which the join of many rows takes them side by side, a
+// row a workgroup, instead of in order, 4 or more rows a workgroup.  Whole
+// calls in order and side by side, us: D = 128, 128 rows a key head, 4000 tokens: 57
+// and 64 with 8 parts, 49 and 47 with 16, 73 and 34 with 64 (30000 tokens, 128
+// parts: 123 and 55); D = 256, 256 rows with 8 parts: 82 and 59.
+constexpr int find_parts(int pad_dim) { return pad_dim == 256 ? 8 : 16; }
+
 template <int DP, int BITS, int NR, int WAVES, int DT>
 hipError_t launch(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_t s)
 {
@@ -1311,10 +1357,18 @@ hipError_t launch(const KvAttentionArgs& a, const KvAttentionPlan& p, hipStream_
     const int used = (int)(rows < kRows ? rows : kRows);
     if constexpr (kMany) {
         constexpr int kAtOnce = kThreads / (DP / 4);
+        // Segments at most.  Where they are few, each is left in many parts,
+        // which a workgroup a row goes through side by side.
+        const int64_t tiles = a.starts ? (rows + kRows - 1) / kRows + a.seqs : a.seqs * ((rows + kRows - 1) / kRows);
+        const int64_t segments = tiles * a.c.heads;
+        if (find_parts(DP) * segments <= p.blocks) {
+            hipLaunchKernelGGL((kv_join_kernel<DP, kRows, DT, true>), dim3((unsigned)segments, used), dim3(kThreads), 0, s, a, p.blocks);
+            return hipGetLastError();
+        }
         hipLaunchKernelGGL((kv_join_rows_kernel<DP, kRows, DT>), dim3(p.blocks, (used + kAtOnce - 1) / kAtOnce),
                            dim3(kThreads), 0, s, a, p.blocks);
     } else {
-        hipLaunchKernelGGL((kv_join_kernel<DP, kRows, DT>), dim3(p.blocks, used), dim3(kThreads), 0, s, a, p.blocks);
+        hipLaunchKernelGGL((kv_join_kernel<DP, kRows, DT, false>), dim3(p.blocks, used), dim3(kThreads), 0, s, a, p.blocks);
     }
     return hipGetLastError();
 }
@@ -1357,9 +1411,15 @@ KvAttentionPlan kv_attention_plan(int64_t n, int seqs, int heads, int kv_heads, 
     p.pad_dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
     const int64_t group = heads / kv_heads;
     const int64_t rows = (n + seqs - 1) / seqs * group;   // of a sequence, on average
-    if (rows <= 16 || (rows <= 32 && p.pad_dim < 256)) {
+    // us, 64 sequences of 4096 tokens, 8 key heads of D = 128 (2 of 256), 4 bits, bf16:
+    //   few rows, two tiles / many, 4 waves of one: 32 rows 86 / 133, 64 rows 161 / 145 (D = 64 and 8 bits: 72 / 77, 101 / 82);
+    //   few rows, one tile / two: 16 rows 75 / 88, 32 rows 126 / 86
+    //   4 waves of one tile / two: 64 rows 145 / 202, 96 rows 255 / 205, 128 rows 266 / 215
+    //   4 waves of two tiles / 8 (16 sequences): 128 rows 87 / 97, 160 rows 125 / 114, 400 rows 212 / 197
+    //   D = 256: few rows / many, 4 waves: 24 rows 66 / 77, 48 rows 99 / 88; 4 waves / 8: 64 rows 97 / 107, 128 rows 148 / 143
+    if (rows <= 32) {
         p.waves = 0;
-        p.tiles = rows <= 16 ? 1 : 2;
+        p.tiles = rows <= 16 || p.pad_dim == 256 ? 1 : 2;
     } else if (p.pad_dim == 256) {
         p.waves = rows <= 64 ? 4 : 8;
         p.tiles = 1;

@@ -325,3 +325,23 @@ def test_refusals():
     # no tokens: an empty result
     out, lse = ca.kv_attention(q[:0], cache, table, lengths, return_lse=True)
     assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+
+
+@pytest.mark.parametrize("dtype,dim,bits", [(torch.bfloat16, 128, 8), (torch.float16, 256, 4), (torch.float32, 64, 4)])
+@pytest.mark.parametrize("counts", [[20], [33, 17], [1, 90]])
+def test_many_rows_of_few_long_sequences(counts, dtype, dim, bits):
+    """Draft trees over long contexts: few segments, each left in many parts by many workgroups."""
+    import coset_amd as ca
+    print(f"few long counts={counts} dim={dim} bits={bits} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(6)
+    page, lengths = 64, [9001, 517][:len(counts)]
+    most = -(-max(lengths) // page)
+    cache = _fill(ca, len(counts) * most, page, 1, dim, bits, 17)
+    rows = []
+    for c in counts:
+        parents = [int(torch.randint(-1, t, (1,), generator=g)) if t else -1 for t in range(c)]
+        m = ca.draft_tree_mask(parents)
+        rows.append(torch.nn.functional.pad(m, (0, 2 - m.shape[1])))
+    table = _table(len(counts), most, cache.pages, 5)
+    _run(ca, cache, lengths, counts, 4, dtype, table, mask=torch.cat(rows))
+    _run(ca, cache, lengths, counts, 8, dtype, table)
